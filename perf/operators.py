@@ -7,8 +7,8 @@ has the cases, draw() more of the same ranges.  exact() restates each operator i
 
 The cache's format.  A group of 32 channels of one key or value is 32 codes of 4 bits (sign, then the magnitudes 0, 0.5,
 1, 1.5, 2, 3, 4, 6) and one power of two, 2^(byte - 127): the smallest with which the group's largest magnitude is at
-most 7 (7 rounds to 6, an error of 1 like that between 4 and 6).  Rounding is to nearest, ties to the even code.  A cache
-is [pages, 2 (keys, values), heads, bytes] of uint8; a page's bytes are its blocks of 16 tokens, each the codes (8 D
+most 7 (7 rounds to 6, an error of 1 like that between 4 and 6).  Rounding is to nearest, ties to the even code.  A
+cache is [pages, 2 (keys, values), heads, bytes] of uint8; a page's bytes are its blocks of 16 tokens, each the codes (8 D
 bytes) and then the scales (D / 2).  Keys: codes [D / 32 groups, 16 tokens, 16 bytes], scales [D / 32, 16].  Values, with
 W = min(D, 128): codes [D / W, 4 quads of tokens, 16, 4 tokens, W / 32 bytes], so that a run of W / 16 channels of four
 consecutive tokens is contiguous, scales [4 quads, D / 32, 4 tokens].  A byte holds channels 2 i (low half) and 2 i + 1.
@@ -55,12 +55,12 @@ def listed():
         # float32 training on rows of no round length, the whole head in the interleaved layout
         dict(name="rotary_f32_odd", kind="rotary", B=3, T=1001, Hq=12, Hk=4, D=64, width=64, interleaved=True,
              dtype="f32", grad=True, far=0),
-        # one new token for each of 64 requests, rotated and stored
-        dict(name="append_decode", kind="append", T=64, Hq=16, Hk=2, D=256, width=64, interleaved=False, page=64,
+        # one new token for each of 64 requests, rotated and stored, each in a page of its own
+        dict(name="append_decode", kind="append", T=64, run=1, Hq=16, Hk=2, D=256, width=64, interleaved=False, page=64,
              dtype="bf16"),
         # a large chunk of prompts, in another shape of head and layout
-        dict(name="append_prompts", kind="append", T=16383, Hq=32, Hk=8, D=128, width=128, interleaved=True, page=16,
-             dtype="bf16"),
+        dict(name="append_prompts", kind="append", T=16383, run=1000, Hq=32, Hk=8, D=128, width=128, interleaved=True,
+             page=16, dtype="bf16"),
         # one request being generated, a short context: latency
         dict(name="attend_one", kind="attend", B=1, ctx=517, new=1, Hq=16, Hk=2, D=256, page=64, dtype="bf16"),
         # a serving batch's decode step over contexts of very different lengths
@@ -88,7 +88,8 @@ def draw(rng):
     dtype = rng.choice(["bf16", "bf16", "f16", "f32"])
     if kind == "plan":
         B = _log(rng, 1, 1024)
-        return dict(kind=kind, B=B, ctx=_log(rng, 1, 32768), new=_log(rng, 1, max(1, min(4096, 120000 // B))), page=page)
+        return dict(kind=kind, B=B, ctx=_log(rng, 1, 32768), new=_log(rng, 1, max(1, min(4096, 120000 // B))),
+                    page=page)
     if kind == "rotary":
         T = _log(rng, 1, 8192)
         most = MOST_ROTARY // ((Hq + Hk) * D * (2 if dtype == "f32" else 1))
@@ -98,7 +99,8 @@ def draw(rng):
                     grad=rng.random() < 0.6, far=rng.choice([0, 0, 200000]))
     if kind == "append":
         T = _log(rng, 1, min(16384, MOST_APPEND // ((Hq + 2 * Hk) * D * DTYPES[dtype].itemsize)))
-        return dict(kind=kind, T=T, Hq=Hq, Hk=Hk, D=D, width=width, interleaved=rng.random() < 0.5, page=page, dtype=dtype)
+        return dict(kind=kind, T=T, run=_log(rng, 1, T), Hq=Hq, Hk=Hk, D=D, width=width, interleaved=rng.random() < 0.5,
+                    page=page, dtype=dtype)
     if kind == "attend":
         new = rng.choice([1, 1, 1, 2, 4, 7])
         ctx = _log(rng, 16, 262144)
@@ -184,10 +186,13 @@ def prepare(case, seed):
         s["positions"] = torch.arange(at, at + c["T"], device="cuda")
         return s
     if c["kind"] == "append":
-        T, page = c["T"], c["page"]
-        pages = -(-2 * T // page) + 1
-        s["cache"] = torch.zeros(pages, 2, c["Hk"], _page_bytes(page, c["D"]), dtype=torch.uint8, device="cuda")
-        s["slots"] = torch.randperm(pages * page, generator=host)[:T].cuda()
+        # runs of consecutive tokens, each run's pages its own and its first token anywhere in the first of them
+        T, run, page = c["T"], c["run"], c["page"]
+        each, runs = -(-(run + page) // page), -(-T // run)
+        s["cache"] = torch.zeros(each * runs, 2, c["Hk"], _page_bytes(page, c["D"]), dtype=torch.uint8, device="cuda")
+        order = torch.randperm(each * runs, generator=host).reshape(runs, each)
+        at = torch.randint(0, page, (runs, 1), generator=host) + torch.arange(run)
+        s["slots"] = (order.gather(1, at // page) * page + at % page).reshape(-1)[:T].cuda()
         # q, k and v are views into one projection's output, as a layer has them
         D, heads = c["D"], c["Hq"] + 2 * c["Hk"]
         qkv = randn(T, heads, D)
@@ -273,7 +278,8 @@ def _places(cache, slots, D):
     p, o = slots.long() // page, slots.long() % page
     t = o % 16
     head = torch.arange(H, device=dev)
-    first = lambda kv: (((p[:, None] * 2 + kv) * H + head) * PB + (o // 16 * 17 * D // 2)[:, None])[..., None]  # noqa: E731
+    block = (o // 16 * 17 * D // 2)[:, None]
+    first = lambda kv: (((p[:, None] * 2 + kv) * H + head) * PB + block)[..., None]  # noqa: E731
     j, g = torch.arange(D // 2, device=dev), torch.arange(D // 32, device=dev)
     W = min(D, 128)
     wb = W // 32
