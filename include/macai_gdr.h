@@ -51,7 +51,7 @@
 extern "C" {
 #endif
 
-#define MACAI_GDR_ABI_VERSION 15
+#define MACAI_GDR_ABI_VERSION 16
 
 /* dtype codes (the rule takes F32 and BF16; the producers also F16) */
 #define MACAI_GDR_F32 0
@@ -262,6 +262,58 @@ int macai_gdr_gates_bwd_typed(const void* b, const void* a, const float* A_log, 
 
 /* Doubles of macai_gdr_gates_bwd_typed's scratch for n elements over H heads. */
 int64_t macai_gdr_gates_partials(int64_t n, int64_t H);
+
+/* ---- the attention layers beside the rule: rotary positions and a paged cache in 4 bits ---- */
+/* (no counterpart in the reference, whose layer package leaves these parts to PyTorch).  dtype F32, BF16 or F16.
+ *
+ * A cache is uint8 [pages, 2 (keys, values), Hk, page * 17 D / 32]: D channels of a token and head are D / 32 groups of 32
+ * codes of 4 bits (E2M1) with a scale byte each, in blocks of 16 tokens whose order is the kernels' own (csrc/gdr_kv4.h);
+ * D 64, 128 or 256, page 16, 32, 64, 128 or 256 tokens.  Token `off` of page p has the slot p * page + off.  A request's
+ * pages are a row of the block table: int32 [B, W], its token t in page blocks[r, t / page].
+ * Row and head strides are in elements and keep 16-byte alignment; a head's D channels are contiguous. */
+
+/* Rotary positions of q [rows, Hq, D] and k [rows, Hk, D] into the dense qo and ko: pairs (a, b) of the first `width`
+ * channels (i and i + width / 2, or 2 i and 2 i + 1 when interleaved) become (a cos - b sin, b cos + a sin) with row i's
+ * position positions[i mod npos] (int32, or int64 when wide) in table [length, width] float32, cos then sin of the width /
+ * 2 angles; transpose turns back (the backward).  width a multiple of 16, D a multiple of 16.  A position outside of the
+ * table gives NaN. */
+int macai_gdr_rotary(const void* q, const void* k, void* qo, void* ko, const float* table, const void* positions,
+                     int64_t rows, int64_t npos, int64_t length, int64_t Hq, int64_t Hk, int64_t D, int64_t width,
+                     int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int32_t wide, int32_t interleaved,
+                     int32_t transpose, int32_t dtype, void* stream);
+
+/* A step's plan from its requests' lengths: request r holds lens[r] tokens and takes add[r] more (negative counts as 0).
+ * starts [B + 1] where its new tokens' rows begin, total [B] = lens + add, positions and slots [tokens] of the rows.  Pages
+ * that the new tokens need come from free_pages [F] in order from head[0] on and are entered in blocks [B, W]; next[0] is
+ * head[0] after them (above F: pages were lacking).  A token without a page (none left, or past the table's W) has the slot
+ * -1, as do rows past the requests' tokens (position 0). */
+int macai_gdr_kv4_plan(const int32_t* lens, const int32_t* add, int32_t* blocks, const int32_t* free_pages,
+                       const int32_t* head, int32_t* starts, int32_t* total, int32_t* positions, int64_t* slots,
+                       int32_t* next, int64_t B, int64_t W, int64_t F, int64_t tokens, int64_t page, void* stream);
+
+/* Stores k and v [rows, Hk, D] at slots [rows] of the cache, k rotated first and rounded to dtype when table is non-NULL
+ * (as macai_gdr_rotary), and writes q [rows, Hq, D] rotated to the dense qo (Hq = 0: no q).  A slot outside of the cache
+ * is not written; two rows with one slot leave either. */
+int macai_gdr_kv4_append(const void* q, const void* k, const void* v, void* qo, uint8_t* cache, const int64_t* slots,
+                         const float* table, const void* positions, int64_t rows, int64_t pages, int64_t page,
+                         int64_t length, int64_t Hq, int64_t Hk, int64_t D, int64_t width, int64_t q_row, int64_t q_head,
+                         int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, int32_t wide, int32_t interleaved,
+                         int32_t dtype, void* stream);
+
+/* The keys and values at slots [rows] as k, v [rows, Hk, D] in dtype; zeros for a slot outside of the cache. */
+int macai_gdr_kv4_read(const uint8_t* cache, const int64_t* slots, void* k, void* v, int64_t rows, int64_t pages,
+                       int64_t page, int64_t Hk, int64_t D, int32_t dtype, void* stream);
+
+/* Attention of q [T, Hq, D] over the cache into the dense o.  Request r's queries are rows starts[r] .. starts[r + 1] (r
+ * alone when starts is NULL, T = B), the last of its lens[r] tokens; query i of n sees the tokens up to lens[r] - n + i.
+ * Query head h reads key head h / (Hq / Hk).  Scores are scaled by `scale`; sums and maxima are float32.  A row that sees
+ * nothing, and rows past starts[B], are zeros; a request with a page number outside of the cache among its tokens' gives
+ * NaN.  workspace: macai_gdr_kv4_attention_workspace bytes, 16-byte aligned. */
+int64_t macai_gdr_kv4_attention_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D);
+int macai_gdr_kv4_attention(const void* q, const uint8_t* cache, const int32_t* blocks, const int32_t* lens,
+                            const int32_t* starts, void* o, void* workspace, int64_t T, int64_t B, int64_t W,
+                            int64_t pages, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t q_row, int64_t q_head,
+                            float scale, int32_t dtype, void* stream);
 
 /* ---- measurement ---- */
 

@@ -13,7 +13,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 KERNELS = os.path.join(CSRC, "gdr_kernels.hip")
 KERNEL_PARTS = 5                  # GDR_PART values of gdr_kernels.hip's C ABI section
-OTHERS = [os.path.join(CSRC, f) for f in ("gdr_forward.hip", "gdr_producers.hip", "gdr_probe.hip")]
+OTHERS = [os.path.join(CSRC, f) for f in ("gdr_forward.hip", "gdr_producers.hip", "gdr_probe.hip", "gdr_cache.hip",
+                                               "gdr_attention.hip")]
 SRCS = [KERNELS] + OTHERS         # the sources the library is built from (besides chunk_bwd8's unit below)
 # chunk_bwd8's translation unit, compiled on its own with LLVM's max-memory-clause machine-scheduling strategy (faster
 # for that kernel; for the whole library it slowed the reverse state pass and grew the float32 state kernels' spills)

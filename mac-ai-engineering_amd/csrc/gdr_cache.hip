@@ -1,0 +1,499 @@
+// What stands around attention over a paged 4-bit cache (gdr_kv4.h has its format): rotary positions, the step's plan,
+// and the cache's writes and reads, for MI355X (gfx950).
+//
+//   rotary   a pair of channels (a, b) at position p becomes (a cos - b sin, b cos + a sin) of the table's angles for
+//            p; a transposed rotation (the backward) takes the sines' negatives.
+//   plan     for requests that hold len tokens and take new more: where each new token's row starts, its position, its
+//            slot in the cache and the pages that the step takes from the free list.
+//   append   rotates q and k, rounds k to its type, and stores k and v in the cache; read gives slots' values back.
+//
+// All are streams: every byte crosses once, and none computes enough to show.
+#include <hip/hip_runtime.h>
+
+#include "gdr_abi.h"
+#include "gdr_common.h"
+#include "gdr_kv4.h"
+
+namespace gdr {
+
+typedef _Float16 f16;
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+
+// 8 values of T (16 or 32 bytes, 16-byte aligned) as floats, and back with one rounding to nearest even.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const f4 a = *reinterpret_cast<const f4*>(p), b = *reinterpret_cast<const f4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a[i], x[i + 4] = b[i];
+  } else {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    const T8 a = *reinterpret_cast<const T8*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f4*>(p) = f4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f4*>(p + 4) = f4{x[4], x[5], x[6], x[7]};
+  } else {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    T8 a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (T)x[i];
+    *reinterpret_cast<T8*>(p) = a;
+  }
+}
+
+// The table's row of a position: cos | sin, width floats; positions int32 or int64.  A position outside of the table has
+// no row: its rotated channels come out NaN.
+struct Rope {
+  const float* table;     // [rows, width], or null: no rotation
+  const void* positions;
+  int64_t rows;
+  int width, wide, interleaved;   // wide: positions are int64
+};
+__device__ __forceinline__ const float* rope_row(const Rope& r, int64_t i) {
+  const int64_t p = r.wide ? reinterpret_cast<const int64_t*>(r.positions)[i]
+                           : (int64_t)reinterpret_cast<const int*>(r.positions)[i];
+  return p >= 0 && p < r.rows ? r.table + p * r.width : nullptr;
+}
+
+// (a, b) turned by an angle: each product rounded on its own, so that every path through this library rotates to the
+// same bits.
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+#pragma clang fp contract(off)
+  const float x = a * c - b * s, y = b * c + a * s;
+  a = x;
+  b = y;
+}
+
+// ---- rotary -------------------------------------------------------------------------------------------------------
+struct RotArgs {
+  const void *q, *k;
+  void *qo, *ko;          // dense [rows, heads, D]
+  Rope rope;
+  int64_t rows, npos;     // row i has position i mod npos
+  int64_t q_row, q_head, k_row, k_head;   // strides in elements
+  int Hq, Hk, D;
+  float sign;             // 1, or -1: the transpose
+};
+
+// A thread takes 16 channels of ROT_HEADS heads of a row that share their angles: a run of 8 and its partners half the
+// width away (interleaved: 16 channels in a row), or 16 that are not rotated.  rotary over 4 x 4,096 tokens, 18 heads of
+// 256, bf16: see the table of cases.
+constexpr int ROT_HEADS = 4;
+template <typename T>
+__global__ void __launch_bounds__(256) rotary_kernel(RotArgs a) {
+  const int units = a.D / 16, heads = a.Hq + a.Hk, groups = (heads + ROT_HEADS - 1) / ROT_HEADS;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int u = (int)(id % units);
+  const int64_t rest = id / units;
+  const int g = (int)(rest % groups);
+  const int64_t row = rest / groups;
+  if (row >= a.rows) return;
+  const int w = a.rope.width, half = w / 2;
+  const bool rot = u < w / 16;
+  const int c0 = rot && !a.rope.interleaved ? u * 8 : u * 16, c1 = rot && !a.rope.interleaved ? half + u * 8 : c0 + 8;
+  float x[ROT_HEADS][2][8];
+#pragma unroll
+  for (int j = 0; j < ROT_HEADS; ++j) {
+    const int h = min(g * ROT_HEADS + j, heads - 1);
+    const T* p = h < a.Hq ? (const T*)a.q + row * a.q_row + h * a.q_head
+                          : (const T*)a.k + row * a.k_row + (h - a.Hq) * a.k_head;
+    load8(p + c0, x[j][0]);
+    load8(p + c1, x[j][1]);
+  }
+  if (rot) {
+    const float* t = rope_row(a.rope, a.npos == a.rows ? row : row % a.npos);
+    float cs[8], sn[8];
+    if (t) {
+      load8(t + u * 8, cs);
+      load8(t + half + u * 8, sn);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) cs[i] = sn[i] = __builtin_nanf("");
+    }
+#pragma unroll
+    for (int j = 0; j < ROT_HEADS; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float s = a.sign * sn[i];
+        if (a.rope.interleaved) turn(x[j][i / 4][2 * i % 8], x[j][i / 4][2 * i % 8 + 1], cs[i], s);
+        else turn(x[j][0][i], x[j][1][i], cs[i], s);
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < ROT_HEADS; ++j) {
+    const int h = g * ROT_HEADS + j;
+    if (h >= heads) break;
+    T* p = h < a.Hq ? (T*)a.qo + (row * a.Hq + h) * a.D : (T*)a.ko + (row * a.Hk + h - a.Hq) * a.D;
+    store8(p + c0, x[j][0]);
+    store8(p + c1, x[j][1]);
+  }
+}
+
+// ---- plan ---------------------------------------------------------------------------------------------------------
+struct PlanArgs {
+  const int *lens, *add;
+  int* blocks;
+  const int *free_, *head;
+  int *starts, *total, *positions, *next;
+  int64_t* slots;
+  int64_t B, W, F, tokens;
+  int page;
+};
+
+// One launch: every workgroup sums over all requests (PLAN_REQ at a time) and finds its own 256 tokens among them, so that
+// nothing waits for another workgroup.  A page is taken by the token that begins it, which also enters it in the table;
+// tokens on a page that was there before read the table, whose old entries no workgroup writes.
+constexpr int PLAN_REQ = 1024;
+__global__ void __launch_bounds__(256) plan_kernel(PlanArgs a) {
+  __shared__ int64_t first[PLAN_REQ + 1];      // where a request's tokens begin
+  __shared__ int64_t taken[PLAN_REQ];          // pages that the requests before it take
+  __shared__ int64_t sums[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t t = (int64_t)blockIdx.x * 256 + tid;
+  const int64_t page = a.page, head = a.head[0];
+  int64_t tok = 0, pages = 0;                  // of the requests before this pass's
+  bool done = t >= a.tokens;
+  for (int64_t r0 = 0; r0 < a.B; r0 += PLAN_REQ) {
+    int64_t n[4], p[4], sn = 0, sp = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = r0 + tid * 4 + i;
+      const int64_t len = r < a.B ? max(a.lens[r], 0) : 0, add = r < a.B ? max(a.add[r], 0) : 0;
+      if (blockIdx.x == 0 && r < a.B) a.total[r] = (int)(len + add);
+      n[i] = sn;
+      p[i] = sp;
+      sn += add;
+      sp += (len + add + page - 1) / page - (len + page - 1) / page;
+    }
+    int64_t in = sn, ip = sp;                  // inclusive sums over the wave, then over the workgroup
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int64_t x = __shfl_up(in, d), y = __shfl_up(ip, d);
+      if (lane >= d) in += x, ip += y;
+    }
+    __syncthreads();                           // the pass before has been read
+    if (lane == 63) sums[0][wave] = in, sums[1][wave] = ip;
+    __syncthreads();
+    int64_t bn = tok, bp = pages;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) bn += sums[0][w], bp += sums[1][w];
+      tok += sums[0][w];
+      pages += sums[1][w];
+    }
+    bn += in - sn;
+    bp += ip - sp;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = r0 + tid * 4 + i;
+      first[tid * 4 + i] = bn + n[i];
+      taken[tid * 4 + i] = bp + p[i];
+      if (blockIdx.x == 0 && r < a.B) a.starts[r] = (int)(bn + n[i]);
+    }
+    if (tid == 0) first[PLAN_REQ] = tok;
+    __syncthreads();
+    if (!done && t < tok) {
+      done = true;
+      int lo = 0, hi = PLAN_REQ - 1;           // the last request that begins at or before t (those after it hold none)
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (first[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      const int64_t r = r0 + lo, len = max(a.lens[r], 0), pos = len + t - first[lo];
+      const int64_t col = pos / page, have = (len + page - 1) / page;
+      int id = -1;
+      if (col < a.W) {
+        if (col >= have) {
+          const int64_t at = head + taken[lo] + col - have;
+          if (at >= 0 && at < a.F) id = a.free_[at];
+          if (pos % page == 0) a.blocks[r * a.W + col] = id;
+        } else {
+          id = a.blocks[r * a.W + col];
+        }
+      }
+      a.positions[t] = (int)pos;
+      a.slots[t] = id < 0 ? -1 : id * page + pos % page;
+    }
+  }
+  if (!done) {                                 // rows past the requests' tokens
+    a.positions[t] = 0;
+    a.slots[t] = -1;
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    a.starts[a.B] = (int)tok;
+    a.next[0] = (int)(head + pages);
+  }
+}
+
+// ---- append and read ------------------------------------------------------------------------------------------------
+struct AppendArgs {
+  const void *q, *k, *v;
+  void* qo;               // dense [rows, Hq, D]; null: only k and v are stored
+  uint8_t* cache;
+  const int64_t* slots;
+  Rope rope;
+  int64_t rows, pages;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // strides in elements
+  int Hq, Hk, D, page;
+};
+
+// The largest of 4 neighbouring lanes (two exchanges inside the quad).
+__device__ __forceinline__ unsigned quad_max(unsigned x) {
+  x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, true));
+  return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));
+}
+
+// A thread takes 8 channels of one head of q, k or v for TT rows; 4 neighbours hold a group of 32.  Rotated channels of
+// the half layout load their partners too (from the first-level cache: another thread's own).
+template <typename T, int TT>
+__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+  const int per = a.D / 8, heads = a.Hq + 2 * a.Hk;
+  const int vec = blockIdx.y * 256 + threadIdx.x;
+  if (vec >= heads * per) return;
+  const int ch = vec % per * 8;
+  int h = vec / per;
+  const int which = h < a.Hq ? 0 : h < a.Hq + a.Hk ? 1 : 2;
+  h -= which == 0 ? 0 : which == 1 ? a.Hq : a.Hq + a.Hk;
+  const T* src = (const T*)(which == 0 ? a.q : which == 1 ? a.k : a.v) +
+                 h * (which == 0 ? a.q_head : which == 1 ? a.k_head : a.v_head);
+  const int64_t step = which == 0 ? a.q_row : which == 1 ? a.k_row : a.v_row;
+  const int w = a.rope.width, half = w / 2;
+  const bool rot = which < 2 && a.rope.table && ch < w, pairs = rot && !a.rope.interleaved;
+  const int partner = ch < half ? ch + half : ch - half;
+  const int64_t row0 = (int64_t)blockIdx.x * TT;
+  float x[TT][8], y[TT][8];
+#pragma unroll
+  for (int i = 0; i < TT; ++i) {
+    const int64_t row = min(row0 + i, a.rows - 1);
+    load8(src + row * step + ch, x[i]);
+    if (pairs) load8(src + row * step + partner, y[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < TT; ++i) {
+    const int64_t row = row0 + i;
+    if (row >= a.rows) break;
+    if (rot) {
+      const float* t = rope_row(a.rope, row);
+      const int at = pairs ? (ch < half ? ch : partner) : ch / 2;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!pairs && (e & 1)) continue;
+        const int j = pairs ? at + e : at + e / 2;
+        const float c = t ? t[j] : __builtin_nanf(""), s = t ? t[half + j] : __builtin_nanf("");
+        if (!pairs) turn(x[i][e], x[i][e + 1], c, s);
+        else if (ch < half) turn(x[i][e], y[i][e], c, s);
+        else turn(y[i][e], x[i][e], c, s);
+      }
+    }
+    if (which == 0) {
+      if (a.qo) store8((T*)a.qo + (row * a.Hq + h) * a.D + ch, x[i]);
+      continue;
+    }
+    unsigned top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[i][e] = (float)(T)x[i][e];                              // as the model's type holds it
+      top = max(top, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);   // a NaN's bits are above an infinity's
+    }
+    const unsigned byte = kv_scale_byte(quad_max(top));
+    const int64_t slot = a.slots[row];
+    if (slot < 0 || slot >= a.pages * a.page) continue;
+    const unsigned word = kv_encode8(x[i], kv_scale(byte));
+    const int off = (int)(slot % a.page), t = off % KV_SUB, g = ch / 32;
+    uint8_t* sub = a.cache + ((slot / a.page * 2 + which - 1) * a.Hk + h) * kv_page_bytes(a.page, a.D) +
+                   off / KV_SUB * kv_sub_bytes(a.D);
+    if (which == 1) {
+      *reinterpret_cast<unsigned*>(sub + kv_key_code(t, ch)) = word;
+      if ((ch & 31) == 0) sub[kv_key_scale(a.D, t, g)] = (uint8_t)byte;
+    } else {
+      uint8_t* p = sub + kv_value_code(a.D, t, ch);
+      if (a.D >= 128) {
+        *reinterpret_cast<unsigned*>(p) = word;
+      } else {
+        *reinterpret_cast<unsigned short*>(p) = (unsigned short)word;
+        *reinterpret_cast<unsigned short*>(p + 8) = (unsigned short)(word >> 16);
+      }
+      if ((ch & 31) == 0) sub[kv_value_scale(a.D, t, g)] = (uint8_t)byte;
+    }
+  }
+}
+
+// Slots' keys and values as T [rows, heads, D] each: 8 channels a thread; a slot outside of the cache reads as zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) read_kernel(const uint8_t* cache, const int64_t* slots, T* k, T* v, int64_t rows,
+                                                   int64_t pages, int Hk, int D, int page) {
+  const int per = D / 8;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int ch = (int)(id % per) * 8;
+  const int64_t rest = id / per;
+  const int hh = (int)(rest % (2 * Hk)), which = hh >= Hk, h = hh - which * Hk;
+  const int64_t row = rest / (2 * Hk);
+  if (row >= rows) return;
+  const int64_t slot = slots[row];
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (slot >= 0 && slot < pages * page) {
+    const int off = (int)(slot % page), t = off % KV_SUB, g = ch / 32;
+    const uint8_t* sub = cache + ((slot / page * 2 + which) * Hk + h) * kv_page_bytes(page, D) +
+                         off / KV_SUB * kv_sub_bytes(D);
+    unsigned word;
+    unsigned byte;
+    if (!which) {
+      word = *reinterpret_cast<const unsigned*>(sub + kv_key_code(t, ch));
+      byte = sub[kv_key_scale(D, t, g)];
+    } else {
+      const uint8_t* p = sub + kv_value_code(D, t, ch);
+      word = D >= 128 ? *reinterpret_cast<const unsigned*>(p)
+                      : *reinterpret_cast<const unsigned short*>(p) |
+                            (unsigned)*reinterpret_cast<const unsigned short*>(p + 8) << 16;
+      byte = sub[kv_value_scale(D, t, g)];
+    }
+    const float s = kv_scale(byte);
+    const unsigned two[4] = {kv_decode2<0>(word, s), kv_decode2<1>(word, s), kv_decode2<2>(word, s),
+                             kv_decode2<3>(word, s)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(two[i] << 16);
+      x[2 * i + 1] = __uint_as_float(two[i] & 0xFFFF0000u);
+    }
+  }
+  store8((which ? v : k) + (row * Hk + h) * D + ch, x);
+}
+
+}  // namespace gdr
+
+// ---- C ABI ----------------------------------------------------------------------------------------------------------
+#define DISPATCH_T(code, ...)                                              \
+  switch (code) {                                                          \
+    case MACAI_GDR_F32: { using PT = float; __VA_ARGS__; } break;          \
+    case MACAI_GDR_BF16: { using PT = gdr::bf16; __VA_ARGS__; } break;     \
+    default: { using PT = gdr::f16; __VA_ARGS__; } break;                  \
+  }
+
+static bool three_types(int32_t t) { return t >= MACAI_GDR_F32 && t <= MACAI_GDR_F16; }
+
+// The strides (elements) of `n` tensors keep 16-byte vectors aligned.
+static bool even_strides(const int64_t* s, int n, int32_t dtype) {
+  const int64_t v = dtype == MACAI_GDR_F32 ? 4 : 8;
+  for (int i = 0; i < n; ++i)
+    if (s[i] % v) return false;
+  return true;
+}
+
+static int check_rope(const char* what, const float* table, const void* positions, int64_t length, int64_t width,
+                      int64_t D) {
+  if (!table || !positions) return fail(MACAI_GDR_EINVAL, "%s: null pointer", what);
+  if (!aligned16(table)) return fail(MACAI_GDR_EINVAL, "%s: pointers must be 16-byte aligned", what);
+  if (width < 16 || width % 16 || width > D)
+    return fail(MACAI_GDR_EUNSUP, "%s: the rotated width must be a multiple of 16 in [16, %lld] (got %lld)", what,
+                (long long)D, (long long)width);
+  if (length < 1) return fail(MACAI_GDR_EINVAL, "%s: the table needs at least one position", what);
+  return MACAI_GDR_OK;
+}
+
+static int check_kv4(const char* what, int64_t pages, int64_t page, int64_t Hk, int64_t D) {
+  if (D != 64 && D != 128 && D != 256)
+    return fail(MACAI_GDR_EUNSUP, "%s: the head width must be 64, 128 or 256 (got %lld)", what, (long long)D);
+  if (page != 16 && page != 32 && page != 64 && page != 128 && page != 256)
+    return fail(MACAI_GDR_EUNSUP, "%s: a page must hold 16, 32, 64, 128 or 256 tokens (got %lld)", what, (long long)page);
+  if (pages < 1 || pages >= INT64_C(1) << 31 || Hk < 1 || Hk > 1024)
+    return fail(MACAI_GDR_EINVAL, "%s: need 1 <= pages < 2^31 and 1 <= key heads <= 1024", what);
+  return MACAI_GDR_OK;
+}
+
+extern "C" {
+
+int macai_gdr_rotary(const void* q, const void* k, void* qo, void* ko, const float* table, const void* positions,
+                     int64_t rows, int64_t npos, int64_t length, int64_t Hq, int64_t Hk, int64_t D, int64_t width,
+                     int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int32_t wide, int32_t interleaved,
+                     int32_t transpose, int32_t dtype, void* stream) {
+  const char* what = "macai_gdr_rotary";
+  if (!three_types(dtype)) return fail(MACAI_GDR_EUNSUP, "%s: dtype codes must be F32, BF16 or F16", what);
+  if (D < 16 || D % 16 || D > 1024)
+    return fail(MACAI_GDR_EUNSUP, "%s: the head width must be a multiple of 16 in [16, 1024] (got %lld)", what, (long long)D);
+  if (rows < 1 || Hq < 0 || Hk < 0 || Hq + Hk < 1 || Hq + Hk > 65536)
+    return fail(MACAI_GDR_EINVAL, "%s: need rows >= 1 and 1 to 65536 heads", what);
+  if (npos < 1 || rows % npos)
+    return fail(MACAI_GDR_EINVAL, "%s: the rows must be a whole number of times the positions", what);
+  if (int rc = check_rope(what, table, positions, length, width, D)) return rc;
+  if ((Hq && (!q || !qo)) || (Hk && (!k || !ko))) return fail(MACAI_GDR_EINVAL, "%s: null pointer", what);
+  const void* ps[] = {q, k, qo, ko};
+  for (const void* p : ps)
+    if (!aligned16(p)) return fail(MACAI_GDR_EINVAL, "%s: pointers must be 16-byte aligned", what);
+  const int64_t strides[] = {q_row, q_head, k_row, k_head};
+  if (!even_strides(strides, 4, dtype)) return fail(MACAI_GDR_EINVAL, "%s: strides must keep 16-byte alignment", what);
+  const int64_t groups = (Hq + Hk + gdr::ROT_HEADS - 1) / gdr::ROT_HEADS;
+  if (rows > (INT64_C(1) << 38) / (groups * (D / 16))) return fail(MACAI_GDR_EINVAL, "%s: too many rows", what);
+  gdr::RotArgs a{q, k, qo, ko, {table, positions, length, (int)width, wide, interleaved}, rows, npos, q_row, q_head, k_row,
+                 k_head, (int)Hq, (int)Hk, (int)D, transpose ? -1.f : 1.f};
+  const dim3 grid((unsigned)((rows * groups * (D / 16) + 255) / 256));
+  DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::rotary_kernel<PT>), grid, dim3(256), 0, (hipStream_t)stream, a))
+  return launched(what);
+}
+
+int macai_gdr_kv4_plan(const int32_t* lens, const int32_t* add, int32_t* blocks, const int32_t* free_pages,
+                       const int32_t* head, int32_t* starts, int32_t* total, int32_t* positions, int64_t* slots,
+                       int32_t* next, int64_t B, int64_t W, int64_t F, int64_t tokens, int64_t page, void* stream) {
+  const char* what = "macai_gdr_kv4_plan";
+  if (page < 1 || page > INT32_MAX) return fail(MACAI_GDR_EINVAL, "%s: need page >= 1", what);
+  if (B < 1 || W < 1 || F < 0 || tokens < 0 || B >= INT32_MAX || W >= INT32_MAX || F >= INT32_MAX || tokens >= INT32_MAX)
+    return fail(MACAI_GDR_EINVAL, "%s: need B >= 1, W >= 1, F >= 0 and tokens >= 0, all below 2^31 - 1", what);
+  if (!lens || !add || !blocks || (F && !free_pages) || !head || !starts || !total || !next ||
+      (tokens && (!positions || !slots)))
+    return fail(MACAI_GDR_EINVAL, "%s: null pointer", what);
+  gdr::PlanArgs a{lens, add, blocks, free_pages, head, starts, total, positions, next, slots, B, W, F, tokens, (int)page};
+  const dim3 grid((unsigned)(tokens ? (tokens + 255) / 256 : 1));
+  hipLaunchKernelGGL(gdr::plan_kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
+  return launched(what);
+}
+
+int macai_gdr_kv4_append(const void* q, const void* k, const void* v, void* qo, uint8_t* cache, const int64_t* slots,
+                         const float* table, const void* positions, int64_t rows, int64_t pages, int64_t page,
+                         int64_t length, int64_t Hq, int64_t Hk, int64_t D, int64_t width, int64_t q_row, int64_t q_head,
+                         int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, int32_t wide, int32_t interleaved,
+                         int32_t dtype, void* stream) {
+  const char* what = "macai_gdr_kv4_append";
+  if (!three_types(dtype)) return fail(MACAI_GDR_EUNSUP, "%s: dtype codes must be F32, BF16 or F16", what);
+  if (int rc = check_kv4(what, pages, page, Hk, D)) return rc;
+  if (rows < 1 || rows >= INT32_MAX || Hq < 0 || Hq > 65536)
+    return fail(MACAI_GDR_EINVAL, "%s: need 1 <= rows < 2^31 and at most 65536 query heads", what);
+  if (!k || !v || !cache || !slots || (Hq && (!q || !qo))) return fail(MACAI_GDR_EINVAL, "%s: null pointer", what);
+  if (table || Hq) {
+    if (int rc = check_rope(what, table, positions, length, width, D)) return rc;
+  }
+  const void* ps[] = {q, k, v, qo, cache};
+  for (const void* p : ps)
+    if (!aligned16(p)) return fail(MACAI_GDR_EINVAL, "%s: pointers must be 16-byte aligned", what);
+  const int64_t strides[] = {q_row, q_head, k_row, k_head, v_row, v_head};
+  if (!even_strides(strides, 6, dtype)) return fail(MACAI_GDR_EINVAL, "%s: strides must keep 16-byte alignment", what);
+  gdr::AppendArgs a{q, k, v, qo, cache, slots, {table, positions, length, (int)width, wide, interleaved}, rows, pages,
+                    q_row, q_head, k_row, k_head, v_row, v_head, (int)Hq, (int)Hk, (int)D, (int)page};
+  const int64_t vecs = ((Hq + 2 * Hk) * (D / 8) + 255) / 256;
+  hipStream_t st = (hipStream_t)stream;
+  DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::append_kernel<PT, 1>), dim3((unsigned)rows, (unsigned)vecs), dim3(256), 0, st, a))
+  return launched(what);
+}
+
+int macai_gdr_kv4_read(const uint8_t* cache, const int64_t* slots, void* k, void* v, int64_t rows, int64_t pages,
+                       int64_t page, int64_t Hk, int64_t D, int32_t dtype, void* stream) {
+  const char* what = "macai_gdr_kv4_read";
+  if (!three_types(dtype)) return fail(MACAI_GDR_EUNSUP, "%s: dtype codes must be F32, BF16 or F16", what);
+  if (int rc = check_kv4(what, pages, page, Hk, D)) return rc;
+  if (rows < 1 || rows >= INT32_MAX) return fail(MACAI_GDR_EINVAL, "%s: need 1 <= rows < 2^31", what);
+  if (!cache || !slots || !k || !v) return fail(MACAI_GDR_EINVAL, "%s: null pointer", what);
+  if (!aligned16(cache) || !aligned16(k) || !aligned16(v))
+    return fail(MACAI_GDR_EINVAL, "%s: pointers must be 16-byte aligned", what);
+  if (rows > (INT64_C(1) << 38) / (2 * Hk * (D / 8))) return fail(MACAI_GDR_EINVAL, "%s: too many rows", what);
+  const dim3 grid((unsigned)((rows * 2 * Hk * (D / 8) + 255) / 256));
+  DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::read_kernel<PT>), grid, dim3(256), 0, (hipStream_t)stream, cache, slots,
+                                       (PT*)k, (PT*)v, rows, pages, (int)Hk, (int)D, (int)page))
+  return launched(what);
+}
+
+}  // extern "C"

@@ -16,7 +16,7 @@ BF16_F32 = 3                          # MACAI_GDR_BF16_F32: bf16 tensors, float3
 OK, EINVAL, EUNSUP, ELAUNCH = 0, 1, 2, 3
 STORE_STATES, NO_OUTPUT = 1, 8
 NOALLOC_SCRATCH_BYTES = 128 << 20     # MACAI_GDR_NOALLOC_SCRATCH_BYTES
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _p, _i64, _i32, _f = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
 # name -> argument types (the order of include/macai_gdr.h)
@@ -45,12 +45,19 @@ SIGNATURES = {
     "macai_gdr_forward": [_p] * 9 + [_i64] * 7 + [_i32, _i32, _f, _i32, _p, _i64, _p],
     "macai_gdr_forward_workspace": [_i64] * 5 + [_i32, _i64],
     "macai_gdr_forward_noalloc": [_p] * 8 + [_i64] * 6 + [_i32, _i32, _f, _i32, _p, _i64, _p],
+    "macai_gdr_rotary": [_p] * 6 + [_i64] * 11 + [_i32] * 4 + [_p],
+    "macai_gdr_kv4_plan": [_p] * 10 + [_i64] * 5 + [_p],
+    "macai_gdr_kv4_append": [_p] * 8 + [_i64] * 14 + [_i32] * 3 + [_p],
+    "macai_gdr_kv4_read": [_p] * 4 + [_i64] * 5 + [_i32, _p],
+    "macai_gdr_kv4_attention_workspace": [_i64] * 5,
+    "macai_gdr_kv4_attention": [_p] * 7 + [_i64] * 10 + [_f, _i32, _p],
     "macai_gdr_probe_stream": [_i32, _p, _p, _i64, _i32, _p],
     "macai_gdr_probe_mfma": [_i32, _i32, _p, _i32, _p],
     "macai_gdr_probe_mfma_flops": [_i32, _i32, _i32],
 }
 # the rest return an int status
-RESTYPES = {"macai_gdr_conv_partials": _i64, "macai_gdr_gates_partials": _i64, "macai_gdr_forward_workspace": _i64, "macai_gdr_probe_mfma_flops": _i64}
+RESTYPES = {"macai_gdr_conv_partials": _i64, "macai_gdr_gates_partials": _i64, "macai_gdr_forward_workspace": _i64,
+            "macai_gdr_kv4_attention_workspace": _i64, "macai_gdr_probe_mfma_flops": _i64}
 
 _lib = None
 _fns = {}        # name -> the library's function object (a lookup per call costs host time on every launch)

@@ -1,0 +1,199 @@
+"""Attention over a paged cache held in 4 bits, and what fills it (the macai_gdr_kv4_* entry points of
+include/macai_gdr.h).  The reference leaves the attention layers' cache to PyTorch.
+
+A layer's cache is one uint8 tensor [pages, 2, key heads, bytes] (kv4_cache): pages of `page` tokens, each token's keys
+and values as groups of 32 codes of 4 bits with a power-of-two scale (17 / 32 of a byte a channel, 3.76 times less than
+bfloat16).  The order of the bytes within a page is the kernels' own; kv4_read gives the values back.
+
+A serving step:
+
+    positions, slots, starts, lens, head = kv4_plan(lens, new, blocks, free, head, tokens, page)     once a step
+    q = kv4_append(q, k, v, cache, slots, rope, positions)                                            a layer
+    o = kv4_attention(q, cache, blocks, lens, starts)                                                 a layer
+
+Everything stays on the device: lengths, tables and slots are never read back, so a step can be captured in a graph.
+"""
+import torch
+
+from ..gated_delta import _native as N
+from ..gated_delta.op import _on
+from ._rotary import DTYPES, _rows, _table_unfit
+
+WIDTHS = (64, 128, 256)
+PAGES = (16, 32, 64, 128, 256)
+
+
+def kv4_cache(pages: int, heads: int, width: int, page: int = 64, device="cuda") -> torch.Tensor:
+    """An empty cache of `pages` pages of `page` tokens for `heads` key heads of `width` channels."""
+    if width not in WIDTHS or page not in PAGES or pages < 1 or heads < 1:
+        raise ValueError(f"macai kv4_cache: need pages, heads >= 1, a width in {WIDTHS} and a page in {PAGES} (got {pages}, "
+                         f"{heads}, {width}, {page})")
+    return torch.zeros(pages, 2, heads, page * 17 * width // 32, dtype=torch.uint8, device=device)
+
+
+def _page_of(cache, width: int, what: str) -> int:
+    """The tokens a page of this cache holds; raises where it is no cache of heads of `width` channels."""
+    if not isinstance(cache, torch.Tensor) or cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[1] != 2:
+        raise ValueError(f"macai {what}: the cache must be a uint8 tensor [pages, 2, heads, bytes] (kv4_cache)")
+    if width not in WIDTHS:
+        raise ValueError(f"macai {what}: the head width must be one of {WIDTHS} (got {width})")
+    page, rest = divmod(cache.shape[3] * 32, 17 * width)
+    if rest or page not in PAGES:
+        raise ValueError(f"macai {what}: {cache.shape[3]} bytes are no page of heads of {width}: a page holds one of {PAGES} "
+                         "tokens")
+    if not cache.is_contiguous() or cache.data_ptr() % 16 or cache.shape[0] < 1 or cache.shape[2] < 1:
+        raise ValueError(f"macai {what}: the cache must be contiguous, 16-byte aligned and not empty")
+    return page
+
+
+def _need(ok: bool, what: str, why: str):
+    if not ok:
+        raise ValueError(f"macai {what}: {why}")
+
+
+def _same_device(what: str, *tensors):
+    dev = tensors[0].device
+    if any(t.device != dev for t in tensors):
+        raise ValueError(f"macai {what}: the tensors must be on one device")
+    if dev.type != "cuda":
+        raise RuntimeError(f"macai's {what} runs on a HIP device (MI355X); got {dev}")
+
+
+def _vector(t, dtype, n, what: str, name: str):
+    """t, checked to be a contiguous tensor of `dtype` [n] (n None: any length)."""
+    _need(isinstance(t, torch.Tensor) and t.dtype == dtype and t.dim() == 1 and (n is None or t.shape[0] == n)
+          and t.is_contiguous(), what, f"{name} must be a contiguous {dtype} tensor [{'n' if n is None else n}]"
+          f" (got {(t.dtype, tuple(t.shape)) if isinstance(t, torch.Tensor) else type(t)})")
+    return t
+
+
+def kv4_plan(lens, new, blocks, free, head, tokens: int, page: int = 64):
+    """One step's bookkeeping on the device, one launch: request r holds lens[r] tokens in the pages blocks[r] (int32 [B,
+    W]) and takes new[r] more, B >= 1.  Pages that the new tokens need are taken from free (int32) in order from head (int32
+    [1], the number taken so far) and entered in blocks, in place.  tokens: the rows of the step's q, at least the sum of new.
+
+    Returns (positions int32 [tokens], slots int64 [tokens], starts int32 [B + 1], total int32 [B] = lens + new, the next
+    head int32 [1]).  Where pages run out or the table is too narrow a token's slot is -1, which kv4_append skips; a next
+    head above len(free) says so.  Rows past the requests' tokens have the slot -1 and position 0.  The inputs other than
+    blocks are left as they are, so a step that is planned again from them comes out the same."""
+    w = "kv4_plan"
+    _need(isinstance(blocks, torch.Tensor) and blocks.dtype == torch.int32 and blocks.dim() == 2 and blocks.is_contiguous()
+          and blocks.numel() > 0, w, "blocks must be a contiguous int32 tensor [B, W] that is not empty")
+    B, W = blocks.shape
+    _vector(lens, torch.int32, B, w, "lens")
+    _vector(new, torch.int32, B, w, "new")
+    _vector(free, torch.int32, None, w, "free")
+    _vector(head, torch.int32, 1, w, "head")
+    _need(tokens >= 0 and page >= 1, w, f"need tokens >= 0 and page >= 1 (got {tokens}, {page})")
+    _same_device(w, blocks, lens, new, free, head)
+    i32 = dict(dtype=torch.int32, device=blocks.device)
+    # one allocation of the int32 outputs
+    out = torch.empty(2 * B + 2 + tokens, **i32)
+    starts, total, nxt, positions = out[:B + 1], out[B + 1:2 * B + 1], out[2 * B + 1:2 * B + 2], out[2 * B + 2:]
+    slots = torch.empty(tokens, dtype=torch.int64, device=blocks.device)
+    with _on(blocks.device):
+        N.call("macai_gdr_kv4_plan", lens.data_ptr(), new.data_ptr(), blocks.data_ptr(), free.data_ptr(), head.data_ptr(),
+               starts.data_ptr(), total.data_ptr(), positions.data_ptr(), slots.data_ptr(), nxt.data_ptr(), B, W,
+               free.shape[0], tokens, page, N.stream_of(blocks))
+    return positions, slots, starts, total, nxt
+
+
+def kv4_append(q, k, v, cache, slots, rope=None, positions=None, interleaved: bool = False):
+    """Stores k and v [T, heads, D] (views into a projection's output are taken as they are) at slots (int64 [T]) of the
+    cache, in place, and returns q [T, query heads, D].  With rope (rotary_table) q and k are rotated to positions (int32 or
+    int64 [T]) first, k rounded to its dtype as rotary returns it; without, q comes back as it is and may be None.  One
+    launch.  Slots outside of the cache (-1) are skipped.  A group of 32 channels that holds an infinity or a NaN reads as
+    NaN.  There is no backward: q, k and v are taken as constants."""
+    w = "kv4_append"
+    for name, t in (("k", k), ("v", v)) if q is None else (("q", q), ("k", k), ("v", v)):
+        _need(isinstance(t, torch.Tensor) and t.dim() == 3, w, f"{name} must be a tensor [T, heads, D]")
+    _need(k.dtype in DTYPES and v.dtype == k.dtype and (q is None or q.dtype == k.dtype), w,
+          "q, k and v must share a dtype among float32, bfloat16, float16")
+    T, Hk, D = k.shape
+    _need(v.shape == k.shape and (q is None or (q.shape[0] == T and q.shape[2] == D)), w,
+          f"q, k, v must be [T, heads, D] of the same tokens and width, k and v alike (got "
+          f"{None if q is None else tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)})")
+    page = _page_of(cache, D, w)
+    _need(cache.shape[2] == Hk, w, f"the cache has {cache.shape[2]} key heads, k and v {Hk}")
+    _vector(slots, torch.int64, T, w, "slots")
+    tensors = [k, v, cache, slots] + ([] if q is None else [q])
+    if rope is not None:
+        _need(q is not None, w, "with a rotary table q is needed")
+        why = _table_unfit(rope, positions, D)
+        _need(why is None, w, str(why))
+        _need(tuple(positions.shape) == (T,) and positions.is_contiguous(), w, f"positions must be contiguous [{T}]")
+        tensors += [rope, positions]
+    _same_device(w, *tensors)
+    qo = q if rope is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if T == 0:
+        return qo
+    k, k_row, k_head = _rows(k, "k")
+    v, v_row, v_head = _rows(v, "v")
+    if rope is None:
+        q_args, r_args, Hq, q_row, q_head, length, width, wide = (None, None), (None, None), 0, 0, 0, 1, 16, 0
+    else:
+        q, q_row, q_head = _rows(q, "q")
+        q_args, r_args, Hq = (q.data_ptr(), qo.data_ptr()), (rope.data_ptr(), positions.data_ptr()), q.shape[1]
+        (length, width), wide = rope.shape, int(positions.dtype == torch.int64)
+    with _on(k.device):
+        N.call("macai_gdr_kv4_append", q_args[0], k.data_ptr(), v.data_ptr(), q_args[1], cache.data_ptr(), slots.data_ptr(),
+               *r_args, T, cache.shape[0], page, length, Hq, Hk, D, width, q_row, q_head, k_row, k_head, v_row, v_head, wide,
+               int(interleaved), N.dtype_code(k.dtype, True), N.stream_of(k))
+    return qo
+
+
+def kv4_read(cache, slots, width: int, dtype=torch.bfloat16):
+    """(k, v) [T, heads, width] of the slots (int64 [T]) in dtype: what kv4_append stored there, exactly as the attention
+    reads it (bfloat16 and float32 hold it exactly).  Slots outside of the cache give zeros."""
+    w = "kv4_read"
+    page = _page_of(cache, width, w)
+    _vector(slots, torch.int64, None, w, "slots")
+    _need(dtype in DTYPES, w, f"dtype must be float32, bfloat16 or float16 (got {dtype})")
+    _same_device(w, cache, slots)
+    T, Hk = slots.shape[0], cache.shape[2]
+    k = torch.empty(T, Hk, width, dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
+    if T:
+        with _on(cache.device):
+            N.call("macai_gdr_kv4_read", cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), T, cache.shape[0],
+                   page, Hk, width, N.dtype_code(dtype, True), N.stream_of(cache))
+    return k, v
+
+
+def kv4_attention(q, cache, blocks, lens, starts=None, scale: float = None):
+    """o [T, query heads, D] in q's dtype: attention of q [T, query heads, D] over the cache.  Request r's tokens are the
+    first lens[r] (int32 [B]) of the pages blocks[r] (int32 [B, W]); its queries are rows starts[r] .. starts[r + 1] (int32
+    [B + 1]; None: one query a request, T = B), the last of those tokens, each seeing the tokens up to its own.  Query head h
+    reads key head h // (query heads / key heads).  scale: D^-1/2 by default.  A row that sees nothing, and rows past the
+    last request's, are zeros.  Table entries past a request's tokens are not read; a page number outside of the cache among
+    them gives that request NaN.  There is no backward: it is the form for serving.
+
+    bfloat16 q: products on bf16 operands (keys and values are exact in them) with 32-bit sums.  float16 and float32 q are
+    taken as two bf16 terms (16 bits)."""
+    w = "kv4_attention"
+    _need(isinstance(q, torch.Tensor) and q.dim() == 3 and q.dtype in DTYPES, w,
+          "q must be a float32, bfloat16 or float16 tensor [T, heads, D]")
+    T, Hq, D = q.shape
+    page = _page_of(cache, D, w)
+    Hk = cache.shape[2]
+    _need(Hq >= Hk and Hq % Hk == 0, w, f"the cache's key heads ({Hk}) must divide the query heads ({Hq})")
+    _need(isinstance(blocks, torch.Tensor) and blocks.dtype == torch.int32 and blocks.dim() == 2 and blocks.is_contiguous(), w,
+          "blocks must be a contiguous int32 tensor [B, W]")
+    B, W = blocks.shape
+    _vector(lens, torch.int32, B, w, "lens")
+    if starts is None:
+        _need(T == B, w, f"without starts every request has one query: {T} rows for {B} requests")
+        _same_device(w, q, cache, blocks, lens)
+    else:
+        _vector(starts, torch.int32, B + 1, w, "starts")
+        _same_device(w, q, cache, blocks, lens, starts)
+    if T == 0 or B == 0 or W == 0:
+        return torch.zeros(T, Hq, D, dtype=q.dtype, device=q.device)
+    o = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+    q, q_row, q_head = _rows(q, "q")
+    work = torch.empty(N.lib().macai_gdr_kv4_attention_workspace(T, B, Hq, Hk, D), dtype=torch.uint8, device=q.device)
+    with _on(q.device):
+        N.call("macai_gdr_kv4_attention", q.data_ptr(), cache.data_ptr(), blocks.data_ptr(), lens.data_ptr(), N.ptr(starts),
+               o.data_ptr(), work.data_ptr(), T, B, W, cache.shape[0], page, Hq, Hk, D, q_row, q_head,
+               D ** -0.5 if scale is None else float(scale), N.dtype_code(q.dtype, True), N.stream_of(q))
+    return o

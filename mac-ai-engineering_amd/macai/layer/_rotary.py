@@ -1,0 +1,164 @@
+"""Rotary positions of the attention layers' queries and keys, one HIP launch each way (entry point macai_gdr_rotary of
+include/macai_gdr.h).  The reference leaves this part to PyTorch.
+
+The first `width` channels of every head are pairs (a, b) -- channels i and i + width / 2, or 2 i and 2 i + 1 when
+interleaved -- turned by the angle of their token's position:
+
+    (a, b) -> (a cos - b sin, b cos + a sin)        float32, rounded once to the input's dtype
+
+and the other channels stay as they are.  The backward is the rotation by the negative angle, in the same kernel.
+The angles come from a table that a model builds once (rotary_table), so nothing is computed from a position at run time
+and scaling for long contexts costs nothing.
+"""
+import math
+
+import torch
+
+from ..gated_delta import _native as N
+from ..gated_delta.op import _on
+
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _frequencies(width: int, base: float, scaling):
+    """(angles per position [width / 2] float64, what cos and sin are multiplied by) under `scaling`."""
+    f = base ** (-torch.arange(0, width, 2, dtype=torch.float64) / width)
+    if scaling is None:
+        return f, 1.0
+    kind, factor = scaling.get("type"), float(scaling.get("factor", 1.0))
+    if factor < 1.0:
+        raise ValueError(f"macai rotary_table: scaling needs a factor >= 1 (got {factor})")
+    if kind == "linear":
+        return f / factor, 1.0
+    if kind == "yarn":
+        # channels that turn more than `fast` times over the original context keep their frequency, those that turn less
+        # than `slow` times are divided by the factor, the ones between are blended linearly in the channel's index
+        original = scaling.get("original")
+        if original is None:
+            raise ValueError("macai rotary_table: yarn scaling needs 'original', the context length trained at")
+        fast, slow = float(scaling.get("fast", 32.0)), float(scaling.get("slow", 1.0))
+        index = lambda turns: width * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+        lo, hi = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), width - 1)
+        ramp = ((torch.arange(width // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        return f * (1 - ramp) + f / factor * ramp, float(scaling.get("attention", 0.1 * math.log(factor) + 1.0))
+    raise ValueError(f"macai rotary_table: scaling type must be 'linear' or 'yarn' (got {kind!r})")
+
+
+def rotary_table(width: int, positions: int, base: float = 10000.0, scaling=None, device="cuda") -> torch.Tensor:
+    """cos | sin of positions 0 .. positions - 1 over the width / 2 angles, [positions, width] float32, formed in float64
+    (an angle of 10^5 turns keeps its float32 accuracy).  scaling: None, {"type": "linear", "factor": f} (positions
+    divided by f) or {"type": "yarn", "factor": f, "original": length, "fast": 32, "slow": 1, "attention": m}."""
+    if width < 16 or width % 16:
+        raise ValueError(f"macai rotary_table: the rotated width must be a positive multiple of 16 (got {width})")
+    if positions < 1:
+        raise ValueError(f"macai rotary_table: need at least one position (got {positions})")
+    f, scale = _frequencies(width, base, scaling)
+    angles = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * f.to(device)
+    return (torch.cat([angles.cos(), angles.sin()], 1) * scale).float()
+
+
+def _rows(t, what: str):
+    """t [..., heads, D] as the kernels take it: (tensor, row stride, head stride) with every leading index one row of a
+    fixed stride, the channels contiguous and 16-byte vectors aligned -- t itself where it is so, as a slice of a
+    projection's output is, a dense copy where not."""
+    shape, s = t.shape, t.stride()
+    v = 16 // t.element_size()
+    if len(shape) < 3:
+        raise ValueError(f"macai: {what} must be [..., tokens, heads, channels] (got {tuple(shape)})")
+    if s[-1] == 1 and s[-2] % v == 0 and s[-3] % v == 0 and t.data_ptr() % 16 == 0:
+        step, rows = s[-3], shape[-3]
+        for n, st in zip(reversed(shape[:-3]), reversed(s[:-3])):
+            if n != 1 and st != step * rows:
+                break
+            rows *= n
+        else:
+            return t, step, s[-2]
+    t = t.contiguous()
+    t = t if t.data_ptr() % 16 == 0 else t.clone()
+    return t, shape[-2] * shape[-1], shape[-1]
+
+
+def _table_unfit(table, positions, width_of: int):
+    """Why a table and positions do not fit heads of width_of channels, or None."""
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype != torch.float32:
+        return "the table must be a float32 tensor [positions, width] (rotary_table)"
+    if table.shape[0] < 1 or table.shape[1] % 16 or not 16 <= table.shape[1] <= width_of:
+        return f"the table's width must be a multiple of 16 up to the head's {width_of} (got {tuple(table.shape)})"
+    if not table.is_contiguous() or table.data_ptr() % 16:
+        return "the table must be contiguous and 16-byte aligned"
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+        return "positions must be an int32 or int64 tensor"
+    return None
+
+
+def _unfit(q, k, table, positions):
+    """Why rotary cannot take these arguments, or None."""
+    if not isinstance(q, torch.Tensor) or not isinstance(k, torch.Tensor):
+        return "q and k must be tensors"
+    if q.dtype not in DTYPES or k.dtype != q.dtype:
+        return f"q and k must share a dtype among float32, bfloat16, float16 (got {q.dtype}, {k.dtype})"
+    if q.dim() < 3 or k.dim() != q.dim() or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+        return f"q and k must be [..., T, heads, D] of the same tokens and width (got {tuple(q.shape)}, {tuple(k.shape)})"
+    if q.shape[-1] % 16 or not 16 <= q.shape[-1] <= 1024:
+        return f"the head width must be a multiple of 16 up to 1024 (got {q.shape[-1]})"
+    if not 1 <= q.shape[-2] + k.shape[-2] <= 65536:
+        return f"need 1 to 65536 heads (got {q.shape[-2]} and {k.shape[-2]})"
+    why = _table_unfit(table, positions, q.shape[-1])
+    if why is not None:
+        return why
+    lead = tuple(q.shape[:-2])
+    if tuple(positions.shape) != lead and tuple(positions.shape) != lead[-1:]:
+        return f"positions must be {lead} or {lead[-1:]} (got {tuple(positions.shape)})"
+    if len({t.device for t in (q, k, table, positions)}) != 1:
+        return "q, k, the table and the positions must be on one device"
+    return None
+
+
+def _rotate(q, k, table, positions, interleaved: bool, back: bool):
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    rows = q.numel() // max(q.shape[-2] * q.shape[-1], 1) if q.shape[-2] else k.numel() // (k.shape[-2] * k.shape[-1])
+    if rows:
+        q, q_row, q_head = _rows(q, "q")
+        k, k_row, k_head = _rows(k, "k")
+        with _on(q.device):
+            N.call("macai_gdr_rotary", q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), table.data_ptr(),
+                   positions.data_ptr(), rows, positions.numel(), table.shape[0], q.shape[-2], k.shape[-2], q.shape[-1],
+                   table.shape[1], q_row, q_head, k_row, k_head, int(positions.dtype == torch.int64), int(interleaved),
+                   int(back), N.dtype_code(q.dtype, True), N.stream_of(q))
+    return qo, ko
+
+
+class Rotary(torch.autograd.Function):
+    """(q, k) rotated (see the module's docstring); the gradients of both in one launch."""
+
+    @staticmethod
+    def forward(ctx, q, k, table, positions, interleaved: bool):
+        ctx.save_for_backward(table, positions)
+        ctx.cfg = (q.shape, k.shape, q.dtype, interleaved)
+        return _rotate(q, k, table, positions, interleaved, False)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        table, positions = ctx.saved_tensors
+        qs, ks, dtype, interleaved = ctx.cfg
+        dq = torch.zeros(qs, dtype=dtype, device=table.device) if dq is None else dq
+        dk = torch.zeros(ks, dtype=dtype, device=table.device) if dk is None else dk
+        dq, dk = _rotate(dq, dk, table, positions, interleaved, True)
+        return (dq if ctx.needs_input_grad[0] else None), (dk if ctx.needs_input_grad[1] else None), None, None, None
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interleaved: bool = False):
+    """(q, k) [..., T, heads, D] with the first table.shape[1] channels of every head rotated to their tokens' positions
+    (int32 or int64, [..., T] or [T]); differentiable in q and k.  Row strides are taken as they are.  A position outside
+    of the table (they are on the device, and not looked at here) gives NaN in the rotated channels."""
+    why = _unfit(q, k, table, positions)
+    if why is not None:
+        raise ValueError("macai rotary: " + why)
+    if not q.is_cuda:
+        raise RuntimeError("macai's rotary positions run on a HIP device (MI355X); got " + str(q.device))
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        return Rotary.apply(q, k, table, positions, bool(interleaved))
+    return _rotate(q, k, table, positions, bool(interleaved), False)

@@ -20,4 +20,7 @@ Pinning (each function's checks live in tests/test_oracle.py):
                            (reference layer/_conv.py, layer/_gates.py); pinned in tests/test_oracle_producers.py
                            against torch's conv1d (groups = channels) + silu, sigmoid and softplus (threshold 20), and
                            the reference's softplus-threshold values.
+  attention.rotate / stored / plan / attention -- the attention layers' operators (no counterpart in the reference);
+                           pinned in tests/test_oracle_attention.py against complex multiplication, a search over the
+                           format's values, the properties of a plan, and torch's softmax.
 """

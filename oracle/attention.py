@@ -1,0 +1,88 @@
+"""Float64 CPU restatement of the attention layers' operators: rotary positions, the paged 4-bit cache's values, a step's
+plan, and attention over a cache (test infrastructure only; see oracle/__init__.py).
+
+Pinned in tests/test_oracle_attention.py against complex multiplication, a search over the format's values, a request by
+request walk, and torch's softmax.
+"""
+import math
+
+import torch
+
+F64 = torch.float64
+MAGNITUDES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def rotate(x, table, positions, interleaved=False, back=False):
+    """The first table.shape[1] channels of every head of x [..., T, H, D] turned by their positions' angles (back: by
+    their negatives); a position outside of the table gives NaN there."""
+    x, w = x.to(F64), table.shape[1]
+    ok = (positions >= 0) & (positions < table.shape[0])
+    cs = table.to(F64)[positions.long().clamp(0, table.shape[0] - 1)]
+    cs = torch.where(ok[..., None], cs, math.nan)
+    cos, sin = cs[..., None, :w // 2], cs[..., None, w // 2:]
+    if back:
+        sin = -sin
+    y = x.clone()
+    a, b = (slice(0, w, 2), slice(1, w, 2)) if interleaved else (slice(0, w // 2), slice(w // 2, w))
+    y[..., a] = x[..., a] * cos - x[..., b] * sin
+    y[..., b] = x[..., b] * cos + x[..., a] * sin
+    return y
+
+
+def stored(x):
+    """x [..., D] as a cache of 4 bits gives it back: per group of 32 channels the scale 2^e, the smallest with the largest
+    magnitude at most 7 2^e (e from -126 to 125), and each value to the nearest of MAGNITUDES times it, ties to the code
+    that is even, at most 6; a group that holds an infinity or a NaN is NaN."""
+    g = x.to(F64).unflatten(-1, (-1, 32))
+    top = g.abs().amax(-1, keepdim=True)
+    bad = ~torch.isfinite(g).all(-1, keepdim=True)
+    e = torch.where(top > 0, torch.ceil(torch.log2(torch.where(bad | (top == 0), 1.0, top) / 7)), -126.0).clamp(-126, 125)
+    y = torch.where(bad, 0.0, g.abs() / 2.0 ** e)
+    mags = torch.tensor(MAGNITUDES, dtype=F64)
+    mid = (mags[1:] + mags[:-1]) / 2
+    code = torch.zeros(y.shape, dtype=torch.long)
+    for i in range(7):                        # a tie at mid[i] goes up where the code above, i + 1, is even
+        code += (y >= mid[i]) if i % 2 == 1 else (y > mid[i])
+    out = torch.where(g < 0, -1.0, 1.0) * mags[code] * 2.0 ** e
+    return torch.where(bad, math.nan, out).flatten(-2)
+
+
+def plan(lens, new, blocks, free, head, tokens, page):
+    """kv4_plan's results as lists, request by request: (positions, slots, starts, total, next head, blocks)."""
+    blocks = [list(r) for r in blocks]
+    W, at = len(blocks[0]), head
+    positions, slots, starts, total = [], [], [0], []
+    for r, (n, m) in enumerate(zip(lens, new)):
+        n, m = max(n, 0), max(m, 0)
+        for col in range(-(-n // page), -(-(n + m) // page)):
+            if col < W:
+                blocks[r][col] = free[at] if 0 <= at < len(free) else -1
+            at += 1
+        for t in range(n, n + m):
+            positions.append(t)
+            p = blocks[r][t // page] if t // page < W else -1
+            slots.append(p * page + t % page if p >= 0 else -1)
+        starts.append(starts[-1] + m)
+        total.append(n + m)
+    pad = max(tokens - len(slots), 0)
+    return (positions + [0] * pad)[:tokens], (slots + [-1] * pad)[:tokens], starts, total, at, blocks
+
+
+def attention(q, k, v, scale):
+    """One request: q [n, Hq, D], the queries of the last n of m tokens; k, v [m, Hk, D].  Returns (o [n, Hq, D], the sum of
+    p |v| [n, Hq, D], the largest sum of |q| |k| scale over a row's keys [n, Hq]); the last two scale error bounds.  A row
+    that sees nothing is zeros."""
+    n, Hq, D = q.shape
+    m, Hk, _ = k.shape
+    o, mag, most = torch.zeros(n, Hq, D, dtype=F64), torch.zeros(n, Hq, D, dtype=F64), torch.zeros(n, Hq, dtype=F64)
+    q, k, v = q.to(F64), k.to(F64), v.to(F64)
+    for i in range(n):
+        see = m - n + i + 1
+        if see <= 0:
+            continue
+        for h in range(Hq):
+            kk, vv = k[:see, h // (Hq // Hk)], v[:see, h // (Hq // Hk)]
+            p = torch.softmax(kk @ q[i, h] * scale, 0)
+            o[i, h], mag[i, h] = p @ vv, p @ vv.abs()
+            most[i, h] = (kk.abs() @ q[i, h].abs()).max() * scale
+    return o, mag, most

@@ -1,0 +1,157 @@
+"""Refusals of the attention layers' operators, all before any launch: the Python functions' and the C ABI's.  CPU only."""
+import pytest
+import torch
+
+from macai.gated_delta import _native as N
+from macai.layer import kv4_append, kv4_attention, kv4_cache, kv4_plan, kv4_read, rotary, rotary_table
+
+I32 = torch.int32
+TABLE = rotary_table(32, 8, device="cpu")
+
+
+def _cache(**kw):
+    return kv4_cache(**dict(dict(pages=3, heads=2, width=64, page=16, device="cpu"), **kw))
+
+
+def _i32(*x):
+    return torch.tensor(x, dtype=I32)
+
+
+@pytest.mark.parametrize("bad", [dict(pages=0), dict(heads=0), dict(width=96), dict(page=24)])
+def test_cache_refusals(bad):
+    with pytest.raises(ValueError, match="macai kv4_cache"):
+        _cache(**bad)
+
+
+def _rotary_args(**kw):
+    return dict(dict(q=torch.zeros(2, 3, 4, 64), k=torch.zeros(2, 3, 2, 64), table=TABLE, positions=torch.zeros(3, dtype=I32)),
+                **kw)
+
+
+@pytest.mark.parametrize("bad,why", [
+    (dict(q=[1]), "tensors"), (dict(q=torch.zeros(2, 3, 4, 64).double()), "dtype"),
+    (dict(k=torch.zeros(2, 3, 2, 64).bfloat16()), "dtype"), (dict(k=torch.zeros(2, 4, 2, 64)), "same tokens"),
+    (dict(k=torch.zeros(2, 3, 2, 32)), "same tokens"), (dict(q=torch.zeros(2, 3, 4, 24), k=torch.zeros(2, 3, 2, 24)), "multiple of 16"),
+    (dict(table=TABLE.double()), "float32"), (dict(table=TABLE[:, :24]), "multiple of 16"), (dict(table=TABLE[::2]), "contiguous"),
+    (dict(q=torch.zeros(2, 3, 4, 16), k=torch.zeros(2, 3, 2, 16)), "up to the head"),
+    (dict(positions=torch.zeros(3)), "int32 or int64"), (dict(positions=torch.zeros(2, dtype=I32)), "positions must be"),
+    (dict(q=torch.zeros(2, 3, 0, 64), k=torch.zeros(2, 3, 0, 64)), "heads")])
+def test_rotary_refusals(bad, why):
+    with pytest.raises(ValueError, match=why):
+        rotary(**_rotary_args(**bad))
+
+
+def test_no_cpu_form():
+    with pytest.raises(RuntimeError, match="HIP device"):
+        rotary(**_rotary_args())
+    with pytest.raises(RuntimeError, match="HIP device"):
+        kv4_append(**_append_args())
+    with pytest.raises(RuntimeError, match="HIP device"):
+        kv4_read(_cache(), torch.zeros(2, dtype=torch.int64), 64)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        kv4_plan(**_plan_args())
+    with pytest.raises(RuntimeError, match="HIP device"):
+        kv4_attention(**_attention_args())
+
+
+def _append_args(**kw):
+    return dict(dict(q=torch.zeros(5, 4, 64), k=torch.zeros(5, 2, 64), v=torch.zeros(5, 2, 64), cache=_cache(),
+                     slots=torch.zeros(5, dtype=torch.int64), rope=TABLE, positions=torch.zeros(5, dtype=I32)), **kw)
+
+
+@pytest.mark.parametrize("bad,why", [
+    (dict(k=None), "k must be"), (dict(v=torch.zeros(5, 2, 64).half()), "dtype"), (dict(q=torch.zeros(4, 4, 64)), "same tokens"),
+    (dict(v=torch.zeros(5, 1, 64)), "alike"), (dict(k=torch.zeros(5, 1, 64), v=torch.zeros(5, 1, 64)), "key heads"),
+    (dict(q=torch.zeros(5, 4, 96), k=torch.zeros(5, 2, 96), v=torch.zeros(5, 2, 96)), "width must be one of"),
+    (dict(cache=torch.zeros(3, 2, 2, 100, dtype=torch.uint8)), "no page"), (dict(cache=_cache().float()), "uint8"),
+    (dict(cache=_cache(pages=6)[::2]), "contiguous"), (dict(slots=torch.zeros(5, dtype=I32)), "slots"),
+    (dict(slots=torch.zeros(4, dtype=torch.int64)), "slots"), (dict(positions=None), "positions"),
+    (dict(positions=torch.zeros(4, dtype=I32)), "positions"), (dict(q=None), "q is needed"),
+    (dict(rope=rotary_table(128, 8, device="cpu")), "up to the head")])
+def test_append_refusals(bad, why):
+    with pytest.raises(ValueError, match=why):
+        kv4_append(**_append_args(**bad))
+
+
+@pytest.mark.parametrize("kw,why", [(dict(width=128), "no page"), (dict(width=32), "width must be one of"),
+                                    (dict(slots=torch.zeros(2, 1, dtype=torch.int64)), "slots"),
+                                    (dict(dtype=torch.float64), "dtype")])
+def test_read_refusals(kw, why):
+    with pytest.raises(ValueError, match=why):
+        kv4_read(**dict(dict(cache=_cache(), slots=torch.zeros(2, dtype=torch.int64), width=64), **kw))
+
+
+def _plan_args(**kw):
+    return dict(dict(lens=_i32(3, 4), new=_i32(1, 1), blocks=torch.zeros(2, 3, dtype=I32), free=_i32(5), head=_i32(0), tokens=2,
+                     page=16), **kw)
+
+
+@pytest.mark.parametrize("bad,why", [
+    (dict(lens=_i32(3)), "lens"), (dict(new=torch.zeros(2)), "new"), (dict(blocks=torch.zeros(2, 3)), "blocks"),
+    (dict(blocks=torch.zeros(3, 2, dtype=I32).T), "blocks"), (dict(blocks=torch.zeros(0, 3, dtype=I32)), "blocks"),
+    (dict(free=torch.zeros(1)), "free"), (dict(head=_i32(0, 0)), "head"), (dict(tokens=-1), "tokens"), (dict(page=0), "page")])
+def test_plan_refusals(bad, why):
+    with pytest.raises(ValueError, match=why):
+        kv4_plan(**_plan_args(**bad))
+
+
+def _attention_args(**kw):
+    return dict(dict(q=torch.zeros(2, 4, 64), cache=_cache(), blocks=torch.zeros(2, 3, dtype=I32), lens=_i32(3, 4)), **kw)
+
+
+@pytest.mark.parametrize("bad,why", [
+    (dict(q=torch.zeros(2, 3, 64)), "divide"), (dict(q=torch.zeros(2, 1, 64)), "divide"), (dict(q=torch.zeros(2, 4, 64).double()), "q must be"),
+    (dict(q=torch.zeros(2, 256)), "q must be"), (dict(q=torch.zeros(3, 4, 64)), "one query"), (dict(lens=_i32(3)), "lens"),
+    (dict(blocks=torch.zeros(2, 3, dtype=torch.int64)), "blocks"), (dict(starts=_i32(0, 1)), "starts"),
+    (dict(q=torch.zeros(2, 4, 128)), "no page")])
+def test_attention_refusals(bad, why):
+    with pytest.raises(ValueError, match=why):
+        kv4_attention(**_attention_args(**bad))
+
+
+def _abi(name, args, **over):
+    a = dict(args)
+    a.update(over)
+    return getattr(N.lib(), "macai_gdr_" + name)(*a.values()), N.lib().macai_gdr_last_error()
+
+
+P = 1 << 20
+ROTARY = dict(q=P, k=P, qo=P, ko=P, table=P, pos=P, rows=4, npos=4, length=8, Hq=2, Hk=1, D=64, width=32, qr=128, qh=64, kr=64,
+              kh=64, wide=0, inter=0, back=0, dtype=1, stream=None)
+PLAN = dict(lens=P, add=P, blocks=P, free=P, head=P, starts=P, total=P, pos=P, slots=P, next=P, B=1, W=1, F=1, tokens=1, page=16,
+            stream=None)
+APPEND = dict(q=P, k=P, v=P, qo=P, cache=P, slots=P, table=P, pos=P, rows=1, pages=1, page=16, length=8, Hq=2, Hk=1, D=64, width=32,
+              qr=128, qh=64, kr=64, kh=64, vr=64, vh=64, wide=0, inter=0, dtype=1, stream=None)
+READ = dict(cache=P, slots=P, k=P, v=P, rows=1, pages=1, page=16, Hk=1, D=64, dtype=1, stream=None)
+ATTEND = dict(q=P, cache=P, blocks=P, lens=P, starts=None, o=P, work=P, T=1, B=1, W=1, pages=1, page=16, Hq=2, Hk=1, D=64, qr=128,
+              qh=64, scale=0.1, dtype=1, stream=None)
+
+
+@pytest.mark.parametrize("name,args,bad,code,why", [
+    ("rotary", ROTARY, dict(dtype=3), "EUNSUP", b"dtype"), ("rotary", ROTARY, dict(D=24), "EUNSUP", b"head width"),
+    ("rotary", ROTARY, dict(width=24), "EUNSUP", b"rotated width"), ("rotary", ROTARY, dict(width=80), "EUNSUP", b"rotated width"),
+    ("rotary", ROTARY, dict(rows=0), "EINVAL", b"rows"), ("rotary", ROTARY, dict(npos=3), "EINVAL", b"whole number"),
+    ("rotary", ROTARY, dict(q=None), "EINVAL", b"null"), ("rotary", ROTARY, dict(table=None), "EINVAL", b"null"),
+    ("rotary", ROTARY, dict(ko=P + 2), "EINVAL", b"aligned"), ("rotary", ROTARY, dict(kh=60), "EINVAL", b"strides"),
+    ("rotary", ROTARY, dict(Hq=0, Hk=0), "EINVAL", b"heads"), ("rotary", ROTARY, dict(length=0), "EINVAL", b"position"),
+    ("kv4_plan", PLAN, dict(B=0), "EINVAL", b"B >= 1"), ("kv4_plan", PLAN, dict(page=0), "EINVAL", b"page"),
+    ("kv4_plan", PLAN, dict(slots=None), "EINVAL", b"null"), ("kv4_plan", PLAN, dict(tokens=2 ** 31), "EINVAL", b"2^31"),
+    ("kv4_append", APPEND, dict(D=96), "EUNSUP", b"head width"), ("kv4_append", APPEND, dict(page=48), "EUNSUP", b"page"),
+    ("kv4_append", APPEND, dict(slots=None), "EINVAL", b"null"), ("kv4_append", APPEND, dict(qo=None), "EINVAL", b"null"),
+    ("kv4_append", APPEND, dict(rows=0), "EINVAL", b"rows"), ("kv4_append", APPEND, dict(pages=0), "EINVAL", b"pages"),
+    ("kv4_append", APPEND, dict(vr=4), "EINVAL", b"strides"), ("kv4_append", APPEND, dict(pos=None), "EINVAL", b"null"),
+    ("kv4_read", READ, dict(dtype=9), "EUNSUP", b"dtype"), ("kv4_read", READ, dict(v=P + 8), "EINVAL", b"aligned"),
+    ("kv4_read", READ, dict(rows=-1), "EINVAL", b"rows"),
+    ("kv4_attention", ATTEND, dict(D=32), "EUNSUP", b"head width"), ("kv4_attention", ATTEND, dict(page=8), "EUNSUP", b"page"),
+    ("kv4_attention", ATTEND, dict(Hq=3, Hk=2), "EINVAL", b"divide"), ("kv4_attention", ATTEND, dict(T=2), "EINVAL", b"one query"),
+    ("kv4_attention", ATTEND, dict(work=None), "EINVAL", b"null"), ("kv4_attention", ATTEND, dict(qr=4), "EINVAL", b"strides"),
+    ("kv4_attention", ATTEND, dict(W=2 ** 28), "EINVAL", b"tokens"), ("kv4_attention", ATTEND, dict(o=P + 4), "EINVAL", b"aligned")])
+def test_abi_refusals(name, args, bad, code, why):
+    rc, msg = _abi(name, args, **bad)
+    assert rc == getattr(N, code) and why in msg, (rc, msg)
+
+
+def test_workspace_sizes():
+    f = N.lib().macai_gdr_kv4_attention_workspace
+    assert f(0, 1, 8, 2, 128) == 0 and f(1, 1, 1, 2, 128) == 0
+    assert f(64, 64, 16, 2, 256) > 0 and f(4096, 4, 16, 2, 256) > 0

@@ -1,0 +1,121 @@
+"""The float64 restatement of the attention layers' operators (oracle/attention.py) against independent forms, and the
+rotary tables against their formulas.  CPU only."""
+import math
+import random
+
+import pytest
+import torch
+
+from macai.layer import rotary_table
+from oracle import attention as A
+
+F64 = torch.float64
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotate_is_a_complex_product(interleaved):
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(5, 3, 64, generator=gen, dtype=F64)
+    table = rotary_table(32, 50, 1000.0, device="cpu")
+    pos = torch.tensor([0, 1, 7, 49, 3])
+    y = A.rotate(x, table, pos, interleaved)
+    for t in range(5):
+        z = torch.complex(table[pos[t], :16].double(), table[pos[t], 16:].double())
+        a, b = (x[t, :, 0:32:2], x[t, :, 1:32:2]) if interleaved else (x[t, :, :16], x[t, :, 16:32])
+        c = torch.complex(a, b) * z
+        ya, yb = (y[t, :, 0:32:2], y[t, :, 1:32:2]) if interleaved else (y[t, :, :16], y[t, :, 16:32])
+        assert torch.allclose(ya, c.real, atol=1e-14) and torch.allclose(yb, c.imag, atol=1e-14)
+    assert torch.equal(y[..., 32:], x[..., 32:])
+    back = A.rotate(y, table, pos, interleaved, back=True)
+    assert torch.allclose(back, x, atol=1e-6)          # the table's cos, sin are float32: their squares sum to 1 to 1e-7
+    assert torch.isnan(A.rotate(x, table, torch.tensor([0, 1, -1, 50, 3]), interleaved)[2:4, :, :32]).all()
+
+
+def test_stored_is_the_nearest_value():
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(40, 32, generator=gen, dtype=F64) * 2.0 ** torch.randint(-20, 20, (40, 1), generator=gen)
+    y = A.stored(x)
+    for g in range(40):
+        top = x[g].abs().max()
+        e = min(e for e in range(-60, 60) if top <= 7 * 2.0 ** e)
+        values = torch.tensor([s * m * 2.0 ** e for m in A.MAGNITUDES for s in (1, -1)], dtype=F64)
+        best = (x[g][:, None] - values).abs().min(1).values
+        assert torch.equal((x[g] - y[g]).abs(), best)
+
+
+def test_stored_ties_ends_and_bad_groups():
+    x = torch.zeros(6, 32, dtype=F64)
+    x[0, :8] = torch.tensor([7.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])       # scale 1: every tie
+    x[1, :2] = torch.tensor([7.5, 0.5])                                         # scale 2: 7.5 is 3.75, 0.5 a tie at 0.25
+    x[2, 3] = math.inf
+    x[3, 5] = math.nan
+    x[5, 0] = 3.3e38                                                            # the largest scale is 2^125
+    y = A.stored(x)
+    assert y[0, :8].tolist() == [6.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0]
+    assert y[1, :2].tolist() == [8.0, 0.0]
+    assert torch.isnan(y[2]).all() and torch.isnan(y[3]).all()
+    assert (y[4] == 0).all() and y[5, 0] == 6 * 2.0 ** 125
+
+
+def test_attention_is_softmax():
+    gen = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(n, h, 16, generator=gen, dtype=F64) for n, h in ((3, 4), (7, 2), (7, 2)))
+    o, mag, most = A.attention(q, k, v, 0.3)
+    for h in range(4):
+        s = q[:, h] @ k[:, h // 2].T * 0.3
+        s = s.masked_fill(torch.arange(7) > 4 + torch.arange(3)[:, None], -math.inf)
+        assert torch.allclose(o[:, h], torch.softmax(s, -1) @ v[:, h // 2], atol=1e-14)
+    assert (mag >= o.abs() - 1e-15).all() and (most > 0).all()
+    o, _, _ = A.attention(q, k[:1], v[:1], 0.3)          # two queries before the first token
+    assert (o[:2] == 0).all() and torch.allclose(o[2], v[0].repeat_interleave(2, 0))
+
+
+def test_plan_gives_every_token_its_own_place():
+    rng = random.Random(4)
+    lens = [rng.randint(0, 70) for _ in range(20)]
+    new = [rng.choice([0, 1, 5, 40]) for _ in lens]
+    pool = list(range(200))
+    rng.shuffle(pool)
+    blocks = [[pool.pop() if c < -(-n // 16) else -1 for c in range(8)] for n in lens]
+    T = sum(new)
+    pos, slots, starts, total, head, after = A.plan(lens, new, blocks, pool, 2, T + 3, 16)
+    assert starts[-1] == T and total == [a + b for a, b in zip(lens, new)]
+    assert len(set(slots[:T])) == T and slots[T:] == [-1] * 3
+    for r in range(20):
+        for i in range(new[r]):
+            t = starts[r] + i
+            assert pos[t] == lens[r] + i and slots[t] == after[r][pos[t] // 16] * 16 + pos[t] % 16
+    assert head == 2 + sum(-(-(a + b) // 16) - -(-a // 16) for a, b in zip(lens, new))
+
+
+def test_rotary_table_formulas():
+    t = rotary_table(16, 200001, 1e6, device="cpu")
+    p, i = 200000, 0
+    assert abs(float(t[p, i]) - math.cos(p)) < 1e-7 and abs(float(t[p, 8]) - math.sin(p)) < 1e-7
+    a = 77 * 1e6 ** (-6 / 16)
+    assert abs(float(t[77, 3]) - math.cos(a)) < 1e-7 and abs(float(t[77, 11]) - math.sin(a)) < 1e-7
+    lin = rotary_table(16, 400, 1e6, scaling=dict(type="linear", factor=4.0), device="cpu")
+    assert torch.allclose(lin[::4], rotary_table(16, 100, 1e6, device="cpu"), atol=1e-7)
+
+
+def test_rotary_table_yarn():
+    """Fast channels as they are, slow ones as under linear scaling, the blend between them, the magnitude."""
+    kw = dict(type="yarn", factor=8.0, original=4096, fast=32.0, slow=1.0)
+    m = 0.1 * math.log(8.0) + 1
+    t = rotary_table(64, 10, 1e4, scaling=kw, device="cpu").double()
+    f = [1e4 ** (-2 * i / 64) for i in range(32)]
+    at = lambda turns: 64 * math.log(4096 / (turns * 2 * math.pi)) / (2 * math.log(1e4))  # noqa: E731
+    lo, hi = math.floor(at(32.0)), math.ceil(at(1.0))
+    assert 0 < lo < hi < 32
+    for i in range(32):
+        r = min(max((i - lo) / (hi - lo), 0), 1)
+        g = f[i] * (1 - r) + f[i] / 8 * r
+        assert abs(float(t[9, i]) - m * math.cos(9 * g)) < 2e-7 and abs(float(t[9, 32 + i]) - m * math.sin(9 * g)) < 2e-7
+    assert torch.allclose(rotary_table(64, 10, 1e4, scaling=dict(kw, attention=1.0), device="cpu").double() * m, t, atol=2e-7)
+
+
+@pytest.mark.parametrize("bad", [dict(width=24), dict(width=0), dict(positions=0), dict(scaling=dict(type="no")),
+                                 dict(scaling=dict(type="linear", factor=0.5)), dict(scaling=dict(type="yarn", factor=2.0))])
+def test_rotary_table_refusals(bad):
+    with pytest.raises(ValueError, match="macai rotary_table"):
+        rotary_table(**dict(dict(width=32, positions=8, device="cpu"), **bad))
