@@ -285,21 +285,8 @@ struct Rows {
               s[b][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[b][w][c * 4 + i], s[b][u], 0, 0, 0);
         }
       }
-    bool nan = false;                            // a value that some row does not see reads as NaN
-    if constexpr (MASKED) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int first = t0 + 16 * u + 4 * h;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-          for (int b = 0; b < NQ; ++b) s[b][u][i] = first + i <= last[b] ? s[b][u][i] : -__builtin_inff();
-          if (first + i >= kend) clear(t, u, i);
-#pragma unroll
-          for (int c = 0; c < TT::NC; ++c) nan |= (t.vs[u][c] >> (8 * i) & 0xFFu) == 0xFFu;
-        }
-      }
-    }
+    unsigned nan[NQ][TT::NC];                    // MASKED: the groups of a row's values that read as NaN
+    if constexpr (MASKED) hide(t, s, nan, t0, kend, h);
     bf16x8 p[NQ][PT];
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
@@ -325,59 +312,66 @@ struct Rows {
           if constexpr (PT == 2) p[b][1][4 * u + i] = (bf16)(e - (float)hi);
         }
     }
-    if (MASKED && __any(nan)) {
-      // 0 times NaN is not 0: a token at a time, its products added only to rows that see it.  Rare; made to be right.
-      for (int one = 0; one < 32; ++one) {
-        const int slot = (one & 16 ? 4 : 0) + (one & 3), quarter = one >> 2 & 3;   // where its values and P are
-        Tile<D> v = t;
-        bf16x8 w[NQ][PT];
-        bool see[NQ];
+    values(t, p);
+    if constexpr (MASKED) {
 #pragma unroll
-        for (int b = 0; b < NQ; ++b) see[b] = t0 + one <= last[b];
+      for (int b = 0; b < NQ; ++b)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int d = 0; d < ND; ++d)             // the lane's channels of a chunk are one group's
+          if (nan[b][d / (ND / TT::NC)] >> (D == 64 ? h / 2 * 8 : 4 * h) & 1u) o[b][d] = f4(__builtin_nanf(""));
+    }
+  }
+
+  // Masks the keys that rows do not see and clears the values past kend and those that read as NaN (0 times NaN is not 0:
+  // a NaN goes to the rows that see it by itself).  nan: bit m of [b][c] is set where the row sees a NaN in the group that
+  // lanes m load of chunk c.
+  __device__ __forceinline__ void hide(Tile<D>& t, f4 (&s)[NQ][2], unsigned (&nan)[NQ][Tile<D>::NC], int t0, int kend, int h) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool keep = h == quarter && 4 * u + i == slot;
-            if (!keep) clear(v, u, i);
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+      for (int c = 0; c < Tile<D>::NC; ++c) nan[b][c] = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = t0 + 16 * u + i, mine = at + 4 * h;
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) s[b][u][i] = mine <= last[b] ? s[b][u][i] : -__builtin_inff();
+#pragma unroll
+        for (int c = 0; c < Tile<D>::NC; ++c) {
+          const bool bad = mine < kend && (t.vs[u][c] >> (8 * i) & 0xFFu) == 0xFFu;
+          const u64 lanes = __ballot(bad);
+          if (lanes) {
 #pragma unroll
             for (int b = 0; b < NQ; ++b)
 #pragma unroll
-              for (int k = 0; k < PT; ++k) w[b][k][4 * u + i] = keep ? p[b][k][4 * u + i] : (bf16)0.f;
+              for (int v = 0; v < 4; ++v)
+                if (at + 4 * v <= last[b]) nan[b][c] |= (unsigned)(lanes >> (16 * v)) & 0xFFFFu;
           }
-        values<true>(v, w, see);
+          if (bad || mine >= kend) {
+            if constexpr (D == 64) t.vc[u][c][i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+            else t.vc[u][c][i] = 0;
+            t.vs[u][c] &= ~(0xFFu << (8 * i));
+          }
+        }
       }
-      return;
-    }
-    bool all[NQ];
-    values<false>(t, p, all);
   }
 
-  // Makes the values of a lane's token (u, i) zeros.
-  __device__ __forceinline__ static void clear(Tile<D>& t, int u, int i) {
-#pragma unroll
-    for (int c = 0; c < Tile<D>::NC; ++c) {
-      if constexpr (D == 64) t.vc[u][c][i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
-      else t.vc[u][c][i] = 0;
-      t.vs[u][c] &= ~(0xFFu << (8 * i));
-    }
-  }
-
-  // O^T += V^T P^T for the tile's 32 tokens; SOME: only to the rows that see them.
-  template <bool SOME, int PT>
-  __device__ __forceinline__ void values(const Tile<D>& t, const bf16x8 (&p)[NQ][PT], const bool (&see)[NQ]) {
+  // O^T += V^T P^T for the tile's 32 tokens.
+  template <int PT>
+  __device__ __forceinline__ void values(const Tile<D>& t, const bf16x8 (&p)[NQ][PT]) {
     constexpr int PER = ND / Tile<D>::NC;
-    two_tiles<0, SOME>(t, p, see);
-    if constexpr (PER > 2) two_tiles<1, SOME>(t, p, see);
+    two_tiles<0>(t, p);
+    if constexpr (PER > 2) two_tiles<1>(t, p);
     if constexpr (PER > 4) {
-      two_tiles<2, SOME>(t, p, see);
-      two_tiles<3, SOME>(t, p, see);
+      two_tiles<2>(t, p);
+      two_tiles<3>(t, p);
     }
   }
 
   // Byte SEL of every token's codes: the lane's channels 2 SEL and 2 SEL + 1 of each run, one output tile each.
-  template <int SEL, bool SOME, int PT>
-  __device__ __forceinline__ void two_tiles(const Tile<D>& t, const bf16x8 (&p)[NQ][PT], const bool (&see)[NQ]) {
+  template <int SEL, int PT>
+  __device__ __forceinline__ void two_tiles(const Tile<D>& t, const bf16x8 (&p)[NQ][PT]) {
     using TT = Tile<D>;
 #pragma unroll
     for (int c = 0; c < TT::NC; ++c) {
@@ -403,18 +397,9 @@ struct Rows {
         const bf16x8 v = __builtin_bit_cast(bf16x8, w);
         const int d = c * (ND / TT::NC) + 2 * SEL + half;
 #pragma unroll
-        for (int b = 0; b < NQ; ++b) {
-          if constexpr (SOME) {
-            f4 z = {0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < NQ; ++b)
 #pragma unroll
-            for (int k = 0; k < PT; ++k) z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[b][k], z, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[b][d][i] += see[b] ? z[i] : 0.f;
-          } else {
-#pragma unroll
-            for (int k = 0; k < PT; ++k) o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[b][k], o[b][d], 0, 0, 0);
-          }
-        }
+          for (int k = 0; k < PT; ++k) o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[b][k], o[b][d], 0, 0, 0);
       }
     }
   }
@@ -436,10 +421,14 @@ __device__ __forceinline__ int channel(int d, int h, int i) {
   return d / RUN * (16 * RUN) + (4 * h + i) * RUN + d % RUN;
 }
 
+// Waves a SIMD holds of the kernel that streams keys for 16 rows: what keeps enough loads in flight (a tile a wave) and
+// fits the registers.
+constexpr int waves_for(int D) { return D == 256 ? 2 : D == 128 ? 3 : 4; }
+
 // KEYS: the workgroup's waves take different keys of the same 16 NQ rows and join their results at the end (few rows);
 // else different rows of the same keys (16 NQ each).
 template <typename T, int D, int NQ, bool KEYS>
-__global__ void __launch_bounds__(64 * AT_WAVES) attend_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(64 * AT_WAVES, KEYS && NQ == 1 ? waves_for(D) : 1) attend_kernel(AttnArgs a) {
   using RT = Rows<T, D, NQ>;
   constexpr int R = 16 * NQ * (KEYS ? 1 : AT_WAVES), STEP = KEYS ? 32 * AT_WAVES : 32, ND = RT::ND;
   constexpr int RUN = D < 128 ? D / 16 : 8;
@@ -487,24 +476,47 @@ __global__ void __launch_bounds__(64 * AT_WAVES) attend_kernel(AttnArgs a) {
 
     RT rw;
     rw.begin(a, x, head, j * R + (KEYS ? 0 : wave * 16 * NQ), G, lane);
-    bool bad = false;
+    // A wave's tiles, the next one's loads in flight while one is worked on, and the page numbers a tile before those.
     const int* table = a.blocks + r * a.W;
     const int64_t pb = kv_page_bytes(a.page, D);
-    for (int t0 = ka + (KEYS ? 32 * wave : 0); t0 < kb; t0 += STEP) {
-      Tile<D> tile;
+    const uint8_t* base = a.cache + (int64_t)head * pb;
+    bool bad = false;
+    int ids[2];
+    const auto look = [&](int t0) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) ids[u] = table[min(t0 + 16 * u, kb - 1) >> a.page_shift];
+    };
+    const auto fetch = [&](int t0, Tile<D>& tile) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int t = t0 + 16 * u;
-        int id = 0;
-        if (t < kb) {
-          id = table[t >> a.page_shift];
-          if ((unsigned)id >= (unsigned)a.pages) bad = true, id = 0;
-        }
-        const uint8_t* k = a.cache + ((int64_t)id * 2 * a.Hk + head) * pb + (t & (a.page - 1)) / KV_SUB * kv_sub_bytes(D);
+        const bool ok = (unsigned)ids[u] < (unsigned)a.pages;
+        bad |= !ok;
+        const uint8_t* k = base + (ok ? ids[u] : 0) * (2 * a.Hk * pb) +
+                           ((t0 + 16 * u) & (a.page - 1)) / KV_SUB * kv_sub_bytes(D);
         load_sub<D>(k, k + a.Hk * pb, tile, u, lane);
       }
-      if (t0 + 32 > min(kmin, kb)) rw.template step<true>(tile, t0, kb, a.scale, lane);
-      else rw.template step<false>(tile, t0, kb, a.scale, lane);
+    };
+    const int full = min(kmin, kb);
+    int t0 = ka + (KEYS ? 32 * wave : 0);
+    Tile<D> tile;
+    if (t0 < kb) {
+      look(t0);
+      fetch(t0, tile);
+      look(t0 + STEP);
+    }
+    while (t0 + 32 <= full) {
+      Tile<D> next;
+      fetch(t0 + STEP, next);
+      look(t0 + 2 * STEP);
+      rw.template step<false>(tile, t0, kb, a.scale, lane);
+      tile = next;
+      t0 += STEP;
+    }
+    while (t0 < kb) {
+      rw.template step<true>(tile, t0, kb, a.scale, lane);
+      t0 += STEP;
+      fetch(t0, tile);
+      look(t0 + STEP);
     }
     rw.end();
     if constexpr (KEYS) {                        // join the waves: 2, 3 into 0, 1, then 1 into 0
@@ -637,7 +649,7 @@ static Shape shape_for(int64_t T, int64_t B, int64_t G) {
   if (rows <= 32) return {2, true};
   return {2, false};
 }
-static int workers_for(const Shape& s) { return s.keys && s.nq == 1 ? 512 : 256; }
+static int workers_for(const Shape& s, int64_t D) { return 256 * (s.keys && s.nq == 1 ? waves_for((int)D) : 1); }
 
 template <typename T, int D>
 static void launch(const Shape& s, const AttnArgs& a, hipStream_t st) {
@@ -668,7 +680,7 @@ extern "C" {
 int64_t macai_gdr_kv4_attention_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D) {
   if (T < 1 || B < 1 || Hk < 1 || Hq < Hk || D < 1) return 0;
   const gdr::Shape s = gdr::shape_for(T, B, Hq / Hk);
-  const int64_t n = gdr::workers_for(s);
+  const int64_t n = gdr::workers_for(s, D);
   return n * (int64_t)sizeof(int4) + 2 * n * s.rows() * (D + 4) * (int64_t)sizeof(float);
 }
 
@@ -698,7 +710,7 @@ int macai_gdr_kv4_attention(const void* q, const uint8_t* cache, const int32_t* 
   if (q_row % v || q_head % v) return fail(MACAI_GDR_EINVAL, "%s: strides must keep 16-byte alignment", what);
   const gdr::Shape s = gdr::shape_for(T, B, Hq / Hk);
   gdr::AttnArgs a{q, o, cache, blocks, lens, starts, nullptr, nullptr, q_row, q_head, T, B, W, pages, (int)Hq, (int)Hk,
-                  (int)page, __builtin_ctzll((unsigned long long)page), gdr::workers_for(s), scale * 1.44269504088896341f};
+                  (int)page, __builtin_ctzll((unsigned long long)page), gdr::workers_for(s, D), scale * 1.44269504088896341f};
   a.records = (int4*)workspace;
   a.part = (float*)((char*)workspace + a.workers * sizeof(int4));
   hipStream_t st = (hipStream_t)stream;
