@@ -22,11 +22,14 @@
 // that covers part of a row group leaves its m, sum and O (32 bits) in the workspace, and a second launch joins them.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cstddef>
 #include <type_traits>
 
 #include "gdr_abi.h"
 #include "gdr_common.h"
 #include "gdr_kv4.h"
+#include "gdr_lds.h"
 
 namespace gdr {
 
@@ -37,6 +40,7 @@ typedef unsigned long long u64;
 
 constexpr int AT_WAVES = 4;
 constexpr float AT_LOWEST = -3.402823466e38f;    // a reference maximum below every score; exp2(-inf - it) is 0
+constexpr int AT_BEGIN = 128;
 constexpr float AT_SLACK = 8.f;                  // how far (log2) scores may pass the reference maximum
 
 struct AttnArgs {
@@ -53,11 +57,15 @@ struct AttnArgs {
 };
 
 // A request as the split sees it.  Costs are in tokens: a row group j of a head costs base + (j + 1) per, the keys its
-// last row sees, rounded up where G does not divide R (a few tokens too many, never too few).
+// last row sees, rounded up where G does not divide R (a few tokens too many, never too few), and AT_BEGIN for what a row
+// group takes besides (its queries, the first loads, its results; without it workgroups with many short row groups ended
+// last: prompts, half the waves' time).
 struct Req {
   int q0, qlen, len, base;                       // first query row, queries, tokens, tokens before the queries
   int groups;                                    // row groups a head
-  __device__ __forceinline__ int64_t cost(int64_t j, int per) const { return j * base + (int64_t)per * j * (j + 1) / 2; }
+  __device__ __forceinline__ int64_t cost(int64_t j, int per) const {
+    return j * (base + AT_BEGIN) + (int64_t)per * j * (j + 1) / 2;
+  }
 };
 
 template <int R>
@@ -168,16 +176,109 @@ __device__ __forceinline__ Place find(const AttnArgs& a, int w, int G, int per, 
   return p;
 }
 
+// A workgroup's stretch, a piece at a time: part or all of the keys of one row group of one head of one request.
+template <int R, int STEP>
+struct Walk {
+  const AttnArgs& a;
+  int w, G, per;
+  Place at;
+  int64_t x0, x1, before, r, u0, u1, stop;       // the line: where the stretch stands and ends, the row group, the piece
+  bool opening;                                  // the stretch's first piece, which may have begun in another
+  int4 record;
+  Req x;
+  int head, j, ka, kb, kmin;                     // row group; keys ka .. kb - 1, of which every row sees those below kmin
+
+  __device__ __forceinline__ Walk(const AttnArgs& args) : a(args) {
+    // neighbours on the line share keys: a stretch of it to each of the 8 dies, whose workgroups are every eighth
+    w = (blockIdx.x & 7) * (a.workers >> 3) + (blockIdx.x >> 3);
+    G = a.Hq / a.Hk;
+    per = (R + G - 1) / G;
+    at = find<R>(a, w, G, per, STEP);
+    x0 = at.share * w;
+    x1 = min(x0 + at.share, at.total);
+    before = at.before;
+    r = at.r;
+    opening = true;
+    record = {0, 0, 0, 0};
+  }
+
+  __device__ __forceinline__ bool next() {
+    while (r < a.B && x0 < x1) {
+      x = request<R>(a, r, G);
+      const int64_t each = x.cost(x.groups, per);   // of a head
+      if (x0 >= before + each * a.Hk) {
+        before += each * a.Hk;
+        ++r;
+        continue;
+      }
+      head = (int)uniform(div64(x0 - before, each));
+      const int64_t y = x0 - before - head * each;
+      int lo = 0, hi = x.groups - 1;             // the row group at y
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (x.cost(mid, per) <= y) lo = mid;
+        else hi = mid - 1;
+      }
+      j = lo;
+      u0 = before + head * each + x.cost(j, per);
+      u1 = before + head * each + x.cost(j + 1, per);
+      stop = min(u1, x1);
+      // the keys: at most the last row's, both ends of a split rounded to whole steps
+      const int rows = min(R, x.qlen * G - j * R), all = x.len - x.qlen + (j * R + rows - 1) / G + 1;
+      kmin = x.len - x.qlen + (j * R) / G + 1;
+      ka = max((int)(x0 - u0) - AT_BEGIN, 0) / STEP * STEP;
+      kb = min(all, stop == u1 ? all : max((int)(stop - u0) - AT_BEGIN, 0) / STEP * STEP);
+      return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ bool whole() const { return x0 == u0 && stop == u1; }
+  __device__ __forceinline__ void done() {
+    if (x0 == u0 && stop != u1)                  // a row group that others go on with begins here
+      record = {(int)r, head * x.groups + j, (int)div64(u1 - 1, at.share), opening ? 1 : 2};
+    opening = false;
+    x0 = stop;
+  }
+  __device__ __forceinline__ void end() const {
+    if (threadIdx.x == 0) a.records[w] = record;
+  }
+};
+
+// Query rows past the last request's have nothing to attend to.
+template <typename T>
+__device__ __forceinline__ void clear_rest(const AttnArgs& a, int D) {
+  if (!a.starts) return;
+  const int64_t used = min((int64_t)max(a.starts[a.B], 0), a.T);
+  for (int64_t t = used + blockIdx.x; t < a.T; t += a.workers)
+    for (int i = threadIdx.x; i < a.Hq * D; i += 64 * AT_WAVES) ((T*)a.o)[t * a.Hq * D + i] = (T)0.f;
+}
+
+// The page numbers of NS blocks of 16 tokens from token t0 on (at most `last`'s), and where a block is.
+template <int NS>
+struct Pages {
+  int id[NS];
+  __device__ __forceinline__ void look(const AttnArgs& a, const int* table, int t0, int last) {
+#pragma unroll
+    for (int u = 0; u < NS; ++u) id[u] = table[min(t0 + 16 * u, last) >> a.page_shift];
+  }
+  // the byte offset of block u of these, of the tokens from t0 on, from a head's keys on; bad: a number out of range
+  __device__ __forceinline__ int64_t at(const AttnArgs& a, int u, int t0, int64_t pb, int sub, bool& bad) const {
+    const bool ok = (unsigned)id[u] < (unsigned)a.pages;
+    bad |= !ok;
+    return (ok ? id[u] : 0) * (2 * a.Hk * pb) + ((t0 + 16 * u) & (a.page - 1)) / KV_SUB * sub;
+  }
+};
+
 // ---- a wave's part -----------------------------------------------------------------------------------------------
 template <int D>
-struct Tile {                                    // 32 tokens' codes and scales as loaded
+struct KvTile {                                    // 32 tokens' codes and scales as loaded
   static constexpr int NC = D < 128 ? 1 : D / 128, NW = D < 128 ? 2 : 4;
   unsigned kc[2][NC][NW], vc[2][NC][NW], ks[2][NC], vs[2][NC];
 };
 
 template <int D>
-__device__ __forceinline__ void load_sub(const uint8_t* k, const uint8_t* v, Tile<D>& t, int s, int lane) {
-  using TT = Tile<D>;
+__device__ __forceinline__ void load_sub(const uint8_t* k, const uint8_t* v, KvTile<D>& t, int s, int lane) {
+  using TT = KvTile<D>;
   const int h = lane >> 4, m = lane & 15;
   if constexpr (D == 64) {
     const u32x2_t x = *reinterpret_cast<const u32x2_t*>(k + (h >> 1) * 256 + m * 16 + (h & 1) * 8);
@@ -263,8 +364,8 @@ struct Rows {
   // which may be anything, are cleared).  P is two terms there: a row of few keys, whose keys are all in such tiles, does
   // not average the roundings of one.
   template <bool MASKED>
-  __device__ __forceinline__ void step(Tile<D>& t, int t0, int kend, float scale, int lane) {
-    using TT = Tile<D>;
+  __device__ __forceinline__ void step(KvTile<D>& t, int t0, int kend, float scale, int lane) {
+    using TT = KvTile<D>;
     constexpr int PT = MASKED ? 2 : TERMS;
     const int h = lane >> 4;
     f4 s[NQ][2];
@@ -325,11 +426,11 @@ struct Rows {
   // Masks the keys that rows do not see and clears the values past kend and those that read as NaN (0 times NaN is not 0:
   // a NaN goes to the rows that see it by itself).  nan: bit m of [b][c] is set where the row sees a NaN in the group that
   // lanes m load of chunk c.
-  __device__ __forceinline__ void hide(Tile<D>& t, f4 (&s)[NQ][2], unsigned (&nan)[NQ][Tile<D>::NC], int t0, int kend, int h) {
+  __device__ __forceinline__ void hide(KvTile<D>& t, f4 (&s)[NQ][2], unsigned (&nan)[NQ][KvTile<D>::NC], int t0, int kend, int h) {
 #pragma unroll
     for (int b = 0; b < NQ; ++b)
 #pragma unroll
-      for (int c = 0; c < Tile<D>::NC; ++c) nan[b][c] = 0;
+      for (int c = 0; c < KvTile<D>::NC; ++c) nan[b][c] = 0;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -338,7 +439,7 @@ struct Rows {
 #pragma unroll
         for (int b = 0; b < NQ; ++b) s[b][u][i] = mine <= last[b] ? s[b][u][i] : -__builtin_inff();
 #pragma unroll
-        for (int c = 0; c < Tile<D>::NC; ++c) {
+        for (int c = 0; c < KvTile<D>::NC; ++c) {
           const bool bad = mine < kend && (t.vs[u][c] >> (8 * i) & 0xFFu) == 0xFFu;
           const u64 lanes = __ballot(bad);
           if (lanes) {
@@ -359,8 +460,8 @@ struct Rows {
 
   // O^T += V^T P^T for the tile's 32 tokens.
   template <int PT>
-  __device__ __forceinline__ void values(const Tile<D>& t, const bf16x8 (&p)[NQ][PT]) {
-    constexpr int PER = ND / Tile<D>::NC;
+  __device__ __forceinline__ void values(const KvTile<D>& t, const bf16x8 (&p)[NQ][PT]) {
+    constexpr int PER = ND / KvTile<D>::NC;
     two_tiles<0>(t, p);
     if constexpr (PER > 2) two_tiles<1>(t, p);
     if constexpr (PER > 4) {
@@ -371,8 +472,8 @@ struct Rows {
 
   // Byte SEL of every token's codes: the lane's channels 2 SEL and 2 SEL + 1 of each run, one output tile each.
   template <int SEL, int PT>
-  __device__ __forceinline__ void two_tiles(const Tile<D>& t, const bf16x8 (&p)[NQ][PT]) {
-    using TT = Tile<D>;
+  __device__ __forceinline__ void two_tiles(const KvTile<D>& t, const bf16x8 (&p)[NQ][PT]) {
+    using TT = KvTile<D>;
 #pragma unroll
     for (int c = 0; c < TT::NC; ++c) {
       unsigned x[8];
@@ -421,6 +522,44 @@ __device__ __forceinline__ int channel(int d, int h, int i) {
   return d / RUN * (16 * RUN) + (4 * h + i) * RUN + d % RUN;
 }
 
+// A wave's 16 NQ rows from lrow0 of the row group on: whole results to o, parts to the workspace.
+template <typename T, int D, int NQ, int R, typename W>
+__device__ __forceinline__ void write_rows(const AttnArgs& a, const W& k, int lrow0, const f4 (&o)[NQ][D / 16],
+                                           const float (&m)[NQ], const float (&l)[NQ], int lane) {
+  constexpr int RUN = D < 128 ? D / 16 : 8, ND = D / 16;
+  typedef T run_t __attribute__((ext_vector_type(RUN)));
+  const int h = lane >> 4, n = lane & 15;
+#pragma unroll
+  for (int b = 0; b < NQ; ++b) {
+    const int lrow = lrow0 + b * 16 + n, row = k.j * R + lrow, i = row / k.G, g = row - i * k.G;
+    if (k.whole()) {
+      if (i >= k.x.qlen) continue;
+      const float inv = l[b] == 0.f ? 0.f : 1.f / l[b];
+      T* p = (T*)a.o + ((int64_t)(k.x.q0 + i) * a.Hq + k.head * k.G + g) * D;
+#pragma unroll
+      for (int c = 0; c < ND / RUN; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          run_t v;
+#pragma unroll
+          for (int f = 0; f < RUN; ++f) v[f] = (T)(o[b][c * RUN + f][e] * inv);
+          *reinterpret_cast<run_t*>(p + channel<D>(c * RUN, h, e)) = v;
+        }
+    } else {
+      float* p = a.part + ((int64_t)(2 * k.w + (k.opening ? 0 : 1)) * R + lrow) * (D + 4);
+#pragma unroll
+      for (int c = 0; c < ND / RUN; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int f = 0; f < RUN; f += 4)
+            *reinterpret_cast<f4*>(p + channel<D>(c * RUN, h, e) + f) =
+                f4{o[b][c * RUN + f][e], o[b][c * RUN + f + 1][e], o[b][c * RUN + f + 2][e], o[b][c * RUN + f + 3][e]};
+      if (h == 0) p[D] = m[b], p[D + 1] = l[b];
+    }
+  }
+}
+
 // Waves a SIMD holds of the kernel that streams keys for 16 rows: what keeps enough loads in flight (a tile a wave) and
 // fits the registers.
 constexpr int waves_for(int D) { return D == 256 ? 2 : D == 128 ? 3 : 4; }
@@ -431,92 +570,47 @@ template <typename T, int D, int NQ, bool KEYS>
 __global__ void __launch_bounds__(64 * AT_WAVES, KEYS && NQ == 1 ? waves_for(D) : 1) attend_kernel(AttnArgs a) {
   using RT = Rows<T, D, NQ>;
   constexpr int R = 16 * NQ * (KEYS ? 1 : AT_WAVES), STEP = KEYS ? 32 * AT_WAVES : 32, ND = RT::ND;
-  constexpr int RUN = D < 128 ? D / 16 : 8;
   __shared__ f4 join_o[KEYS ? 2 : 1][KEYS ? NQ * ND : 1][64];
   __shared__ float join_m[KEYS ? AT_WAVES : 1][NQ][16], join_l[KEYS ? AT_WAVES : 1][NQ][16];
   const int lane = threadIdx.x & 63, h = lane >> 4, n = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = a.Hq / a.Hk, per = (R + G - 1) / G;
-  const int w = blockIdx.x;
-  const Place at = find<R>(a, w, G, per, STEP);
-  int4 record = {0, 0, 0, 0};
-  if (a.starts) {                                // query rows past the last request's have nothing to attend to
-    const int64_t used = min((int64_t)max(a.starts[a.B], 0), a.T);
-    for (int64_t t = used + w; t < a.T; t += a.workers)
-      for (int i = threadIdx.x; i < a.Hq * D; i += 64 * AT_WAVES) ((T*)a.o)[t * a.Hq * D + i] = (T)0.f;
-  }
-  int64_t x0 = at.share * w;
-  const int64_t x1 = min(x0 + at.share, at.total);
-  int64_t before = at.before;
-  bool opening = true;                           // the stretch's first piece: it may have begun in another
-  for (int64_t r = at.r; r < a.B && x0 < x1;) {
-    const Req x = request<R>(a, r, G);
-    const int64_t each = x.cost(x.groups, per);  // of a head
-    if (x0 >= before + each * a.Hk) {
-      before += each * a.Hk;
-      ++r;
-      continue;
-    }
-    const int head = (int)uniform(div64(x0 - before, each));
-    const int64_t y = x0 - before - head * each;
-    int j = 0;
-    for (int lo = 0, hi = x.groups - 1;; ) {     // the row group at y
-      if (lo >= hi) { j = lo; break; }
-      const int mid = (lo + hi + 1) / 2;
-      if (x.cost(mid, per) <= y) lo = mid;
-      else hi = mid - 1;
-    }
-    const int64_t u0 = before + head * each + x.cost(j, per), u1 = before + head * each + x.cost(j + 1, per);
-    const int64_t stop = min(u1, x1);
-    // the keys: the last row's at the most, both ends of a split rounded to whole steps
-    const int rows = min(R, x.qlen * G - j * R), kall = x.len - x.qlen + (j * R + rows - 1) / G + 1;
-    const int kmin = x.len - x.qlen + (j * R) / G + 1;          // keys that every row sees
-    int ka = (int)(x0 - u0) / STEP * STEP, kb = stop == u1 ? kall : (int)(stop - u0) / STEP * STEP;
-    kb = min(kb, kall);
-
+  Walk<R, STEP> k(a);
+  clear_rest<T>(a, D);
+  const int64_t pb = kv_page_bytes(a.page, D);
+  while (k.next()) {
     RT rw;
-    rw.begin(a, x, head, j * R + (KEYS ? 0 : wave * 16 * NQ), G, lane);
+    rw.begin(a, k.x, k.head, k.j * R + (KEYS ? 0 : wave * 16 * NQ), k.G, lane);
     // A wave's tiles, the next one's loads in flight while one is worked on, and the page numbers a tile before those.
-    const int* table = a.blocks + r * a.W;
-    const int64_t pb = kv_page_bytes(a.page, D);
-    const uint8_t* base = a.cache + (int64_t)head * pb;
+    const int* table = a.blocks + k.r * a.W;
+    const uint8_t* base = a.cache + (int64_t)k.head * pb;
     bool bad = false;
-    int ids[2];
-    const auto look = [&](int t0) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) ids[u] = table[min(t0 + 16 * u, kb - 1) >> a.page_shift];
-    };
-    const auto fetch = [&](int t0, Tile<D>& tile) {
+    Pages<2> pages;
+    const auto fetch = [&](int t0, KvTile<D>& tile) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const bool ok = (unsigned)ids[u] < (unsigned)a.pages;
-        bad |= !ok;
-        const uint8_t* k = base + (ok ? ids[u] : 0) * (2 * a.Hk * pb) +
-                           ((t0 + 16 * u) & (a.page - 1)) / KV_SUB * kv_sub_bytes(D);
-        load_sub<D>(k, k + a.Hk * pb, tile, u, lane);
+        const uint8_t* p = base + pages.at(a, u, t0, pb, kv_sub_bytes(D), bad);
+        load_sub<D>(p, p + a.Hk * pb, tile, u, lane);
       }
+      pages.look(a, table, t0 + STEP, k.kb - 1);
     };
-    const int full = min(kmin, kb);
-    int t0 = ka + (KEYS ? 32 * wave : 0);
-    Tile<D> tile;
-    if (t0 < kb) {
-      look(t0);
+    const int full = min(k.kmin, k.kb);
+    int t0 = k.ka + (KEYS ? 32 * wave : 0);
+    KvTile<D> tile;
+    if (t0 < k.kb) {
+      pages.look(a, table, t0, k.kb - 1);
       fetch(t0, tile);
-      look(t0 + STEP);
     }
     while (t0 + 32 <= full) {
-      Tile<D> next;
+      KvTile<D> next;
       fetch(t0 + STEP, next);
-      look(t0 + 2 * STEP);
-      rw.template step<false>(tile, t0, kb, a.scale, lane);
+      rw.template step<false>(tile, t0, k.kb, a.scale, lane);
       tile = next;
       t0 += STEP;
     }
-    while (t0 < kb) {
-      rw.template step<true>(tile, t0, kb, a.scale, lane);
+    while (t0 < k.kb) {
+      rw.template step<true>(tile, t0, k.kb, a.scale, lane);
       t0 += STEP;
       fetch(t0, tile);
-      look(t0 + STEP);
     }
     rw.end();
     if constexpr (KEYS) {                        // join the waves: 2, 3 into 0, 1, then 1 into 0
@@ -561,53 +655,378 @@ __global__ void __launch_bounds__(64 * AT_WAVES, KEYS && NQ == 1 ? waves_for(D) 
 #pragma unroll
       for (int b = 0; b < NQ; ++b) rw.l[b] = __builtin_nanf("");
     }
-    const bool whole = x0 == u0 && stop == u1;
-    if (!KEYS || wave == 0) {
+    if (!KEYS || wave == 0) write_rows<T, D, NQ, R>(a, k, KEYS ? 0 : wave * 16 * NQ, rw.o, rw.m, rw.l, lane);
+    k.done();
+  }
+  k.end();
+}
+
+// ---- many rows: chunks of prompts ------------------------------------------------------------------------------------
+// Bound by the matrix cores, so decoding has to leave their way.  A workgroup's four waves take 32 rows each of the same
+// keys, KT at a time (two workgroups a CU at heads of 128, one wave's products over another's softmax):
+//   scores   v_mfma_scale_f32_16x16x128_f8f6f4 takes a key's codes and scale bytes as they lie in the cache, nothing is
+//            decoded.  A bf16 query is the sum of two FP8 (E4M3) terms, 4 bits of its 8 each, with a power of two for each
+//            group of 32 channels and term: exact for values down to 2^-13 of their group's largest, 2^-21 of the largest
+//            below.  Two such products of 128 channels take half the time of the four bf16 ones.
+//   values   decoded once for the workgroup, a quarter each, into LDS in the order that the second product's operand has
+//            (contiguous 16-byte reads, no bank conflict); two buffers, one barrier a tile.
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
+template <int D>
+struct Prompt {
+  static constexpr int NQ = 2, NC = D / 128, KT = D == 256 ? 32 : 64, NS = KT / 16, KB = KT / 32, ND = D / 16;
+  static constexpr int R = 16 * NQ * AT_WAVES;
+  static constexpr int RING = 5;                 // tiles' codes in LDS: the one in use, the next, and three on their way
+  static_assert(NS * NC == AT_WAVES, "a wave copies and decodes one block of 16 tokens and 128 channels of a tile");
+  struct Raw {                                   // a tile as it lies in the cache: block u, chunk c at [u NC + c]
+    unsigned k[AT_WAVES][64][4], v[AT_WAVES][64][4];
+    uint8_t scales[AT_WAVES][256];               // of block u at [u NC]: keys' D / 2 bytes, values' D / 2
+  };
+  struct Shared {
+    Raw raw[RING];
+    unsigned operands[2][KB * ND][64][4];        // V^T
+    u64 nans[2][AT_WAVES][4];
+    int lost;
+  };
+  i32x8_t q[NQ][NC][2];                          // a row's FP8 terms: channels 128 c + 16 h + 0..15, + 64 + 0..15
+  unsigned qs[NQ];                               // their scales for group 4 c + h: bytes 2 c (high term), 2 c + 1 (low)
+  f4 o[NQ][ND];
+  float m[NQ], l[NQ];
+  int last[NQ];
+
+  template <int C>
+  __device__ __forceinline__ void begin_chunk(const bf16* p, int b, bool there, int lane) {
+    const int h = lane >> 4;
+    float v[2][8], w[2][8];
+    float top[2] = {0.f, 0.f};
+    int e[2];
 #pragma unroll
-      for (int b = 0; b < NQ; ++b) {
-        const int lrow = (KEYS ? 0 : wave * 16 * NQ) + b * 16 + n, row = j * R + lrow, i = row / G, g = row - i * G;
-        if (whole) {
-          if (i >= x.qlen) continue;
-          const float inv = rw.l[b] == 0.f ? 0.f : 1.f / rw.l[b];
-          T* p = (T*)a.o + ((int64_t)(x.q0 + i) * a.Hq + head * G + g) * D;
+    for (int part = 0; part < 2; ++part) {
+      load_f8(p + C * 128 + part * 64 + 16 * h, v[part]);
+      load_f8(p + C * 128 + part * 64 + 16 * h + 8, w[part]);
+      unsigned bits = 0;
 #pragma unroll
-          for (int c = 0; c < ND / RUN; ++c)
+      for (int i = 0; i < 8; ++i) {
+        if (!there) v[part][i] = w[part][i] = 0.f;
+        bits = max(bits, max(__float_as_uint(v[part][i]) & 0x7FFFFFFFu, __float_as_uint(w[part][i]) & 0x7FFFFFFFu));
+      }
+      bits = max(bits, (unsigned)__shfl_xor((int)bits, 16));       // the group's other half
+      e[part] = bits >= 0x7F800000u ? 255 : max((int)(bits >> 23) - 7, 8);
+      const float down = __uint_as_float((unsigned)(254 - min(e[part], 253)) << 23);   // 2^(127 - e): values up to 256
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              typedef T TR __attribute__((ext_vector_type(RUN)));
-              TR v;
+      for (int i = 0; i < 4; ++i) {              // 4 bytes from 4 channels
+        const float x[4] = {(i < 2 ? v : w)[part][4 * (i & 1)] * down, (i < 2 ? v : w)[part][4 * (i & 1) + 1] * down,
+                            (i < 2 ? v : w)[part][4 * (i & 1) + 2] * down, (i < 2 ? v : w)[part][4 * (i & 1) + 3] * down};
+        int hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], hi, true);
+        int lo = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - __builtin_amdgcn_cvt_f32_fp8(hi, 0)) * 16.f,
+                                                 (x[1] - __builtin_amdgcn_cvt_f32_fp8(hi, 1)) * 16.f, 0, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - __builtin_amdgcn_cvt_f32_fp8(hi, 2)) * 16.f,
+                                             (x[3] - __builtin_amdgcn_cvt_f32_fp8(hi, 3)) * 16.f, lo, true);
+        q[b][C][0][part * 4 + i] = hi;
+        q[b][C][1][part * 4 + i] = lo;
+      }
+    }
+    // lane quarter h gives group 4 C + h's scale: it is with quarters 2 h, 2 h + 1 of the first part, or of the second
+    const int from = (lane & 15) + 32 * (h & 1), e0 = __shfl(e[0], from), e1 = __shfl(e[1], from), mine = h < 2 ? e0 : e1;
+    qs[b] |= (unsigned)(mine | (mine == 255 ? 255 : mine - 4) << 8) << (16 * C);
+  }
+
+  __device__ __forceinline__ void begin(const AttnArgs& a, const Req& x, int head, int row0, int G, int lane) {
+    const int n = lane & 15;
 #pragma unroll
-              for (int f = 0; f < RUN; ++f) v[f] = (T)(rw.o[b][c * RUN + f][e] * inv);
-              *reinterpret_cast<TR*>(p + channel<D>(c * RUN, h, e)) = v;
-            }
-        } else {
-          float* p = a.part + ((int64_t)(2 * w + (opening ? 0 : 1)) * R + lrow) * (D + 4);
+    for (int b = 0; b < NQ; ++b) {
+      const int row = row0 + b * 16 + n, i = row / G, g = row - i * G;
+      const bool there = i < x.qlen;
+      last[b] = there ? x.len - x.qlen + i : -1;
+      const bf16* p = (const bf16*)a.q + (x.q0 + (there ? i : 0)) * a.q_row + (int64_t)(head * G + g) * a.q_head;
+      qs[b] = 0;
+      begin_chunk<0>(p, b, there, lane);
+      if constexpr (NC == 2) begin_chunk<1>(p, b, there, lane);
 #pragma unroll
-          for (int c = 0; c < ND / RUN; ++c)
+      for (int d = 0; d < ND; ++d) o[b][d] = f4{0.f, 0.f, 0.f, 0.f};
+      m[b] = AT_LOWEST;
+      l[b] = 0.f;
+    }
+  }
+
+  // Starts the copy of the wave's share of a tile (3 loads) into the Raw at LDS address `to`: its block's codes, and that
+  // block's 16 tokens' scales.  Not seen by the compiler, which would have every LDS access wait for it; waited for by
+  // wait_vmcnt before a barrier.
+  __device__ __forceinline__ static void copy(const uint8_t* keys, const uint8_t* values, unsigned to, int wave, int lane) {
+    const int c = wave % NC;
+    dma<16>(keys + c * 1024, to + offsetof(Raw, k) + wave * 1024, lane * 16, 1024);
+    dma<16>(values + c * 1024, to + offsetof(Raw, v) + wave * 1024, lane * 16, 1024);
+    // lanes below D / 8 take the keys' scales, the next D / 8 the values' (as an offset from the keys'), the rest repeat
+    const int i = lane & (D / 4 - 1), far = (int)(values - keys);
+    dma<4>(keys + 8 * D, to + offsetof(Raw, scales) + wave * 256, i < D / 8 ? i * 4 : far + (i - D / 8) * 4, far + D / 2);
+  }
+  // lane l's SIZE bytes at from + off to LDS address to + SIZE l; nothing at or past from + bytes is read.
+  template <int SIZE>
+  __device__ __forceinline__ static void dma(const uint8_t* from, unsigned to, int off, int bytes) {
+    const u64 g = (u64)from;
+    const u32x4_t rs = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)g),
+                        (unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned)(g >> 32) & 0xFFFFu)), (unsigned)bytes,
+                        0x00020000u};
+    const unsigned lds = __builtin_amdgcn_readfirstlane((int)to);
+    // The compiler does not see into the asm, so the wait states that it would insert are here: 5 between a VALU write of
+    // an SGPR (readfirstlane may be the instruction before) and a vector-memory read of it, 1 after an SALU write of M0.
+    if constexpr (SIZE == 16)
+      asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(off), "s"(rs), "{m0}"(lds) : "memory");
+    else
+      asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" : : "v"(off), "s"(rs), "{m0}"(lds) : "memory");
+  }
+
+  // Decodes the wave's block of a tile's values, tokens from t on, into a buffer of operands.  masked: values past kend are
+  // cleared, and those that read as NaN, whose places are left in `nan` (lane masks of tokens i) for every wave.
+  __device__ __forceinline__ static void stage_values(const Raw& raw, unsigned (*buf)[64][4], u64* nan, int wave, int t,
+                                                      bool masked, int kend, int lane) {
+    const int h = lane >> 4, u = wave / NC, c = wave % NC;
+    const u32x4_t codes = *reinterpret_cast<const u32x4_t*>(&raw.v[wave][lane][0]);
+    unsigned vs = *reinterpret_cast<const unsigned*>(&raw.scales[u * NC][D / 2 + h * (D / 8) + (4 * c + ((lane & 15) >> 2)) * 4]);
+    unsigned vc[4] = {codes[0], codes[1], codes[2], codes[3]};
+    if (masked) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int f = 0; f < RUN; f += 4)
-                *reinterpret_cast<f4*>(p + channel<D>(c * RUN, h, e) + f) =
-                    f4{rw.o[b][c * RUN + f][e], rw.o[b][c * RUN + f + 1][e], rw.o[b][c * RUN + f + 2][e],
-                       rw.o[b][c * RUN + f + 3][e]};
-          if (h == 0) p[D] = rw.m[b], p[D + 1] = rw.l[b];
+      for (int i = 0; i < 4; ++i) {
+        const bool past = t + 4 * h + i >= kend, bad = !past && (vs >> (8 * i) & 0xFFu) == 0xFFu;
+        const u64 lanes = __ballot(bad);
+        if (lane == 0) nan[i] = lanes;
+        if (past || bad) {
+          vc[i] = 0;
+          vs &= ~(0xFFu << (8 * i));
         }
       }
     }
-    if (x0 == u0 && stop != u1)                  // this workgroup begins a row group that others go on with
-      record = {(int)r, head * x.groups + j, (int)div64(u1 - 1, at.share), opening ? 1 : 2};
-    opening = false;
-    x0 = stop;
+    stage_two<0>(vc, vs, buf, u, c, lane);
+    stage_two<1>(vc, vs, buf, u, c, lane);
+    stage_two<2>(vc, vs, buf, u, c, lane);
+    stage_two<3>(vc, vs, buf, u, c, lane);
   }
-  if (threadIdx.x == 0) a.records[w] = record;
+  template <int SEL>
+  __device__ __forceinline__ static void stage_two(const unsigned (&vc)[4], unsigned vs, unsigned (*buf)[64][4], int u, int c,
+                                                   int lane) {
+    unsigned x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = kv_decode2<SEL>(vc[i], kv_scale(vs >> (8 * i) & 0xFFu));
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const unsigned sel = half ? 0x07060302u : 0x05040100u;
+      const u32x2_t w = {__builtin_amdgcn_perm(x[1], x[0], sel), __builtin_amdgcn_perm(x[3], x[2], sel)};
+      *reinterpret_cast<u32x2_t*>(&buf[u / 2 * ND + c * 8 + 2 * SEL + half][lane][2 * (u & 1)]) = w;
+    }
+  }
+
+  // S^T of the tile's keys; consecutive products go to different sums.
+  __device__ __forceinline__ void scores(const Raw& raw, f4 (&s)[NQ][NS], int lane) const {
+    u32x4_t x[NS];
+    int ks[NS];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+#pragma unroll
+      for (int u = 0; u < NS; ++u) {
+        x[u] = *reinterpret_cast<const u32x4_t*>(&raw.k[u * NC + c][lane][0]);
+        ks[u] = raw.scales[u * NC][64 * c + lane];
+      }
+      if (c == 0) products<0>(x, ks, s);
+      else products<1>(x, ks, s);
+    }
+  }
+  template <int C>
+  __device__ __forceinline__ void products(const u32x4_t (&x)[NS], const int (&ks)[NS], f4 (&s)[NQ][NS]) const {
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
+        const i32x8_t k = {(int)x[u][0], (int)x[u][1], (int)x[u][2], (int)x[u][3], 0, 0, 0, 0};
+        const f4 from = C == 0 ? f4{0.f, 0.f, 0.f, 0.f} : s[b][u];
+        s[b][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q[b][C % NC][0], from, 4, 0, 0, ks[u], 2 * C, (int)qs[b]);
+      }
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
+        const i32x8_t k = {(int)x[u][0], (int)x[u][1], (int)x[u][2], (int)x[u][3], 0, 0, 0, 0};
+        s[b][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q[b][C % NC][1], s[b][u], 4, 0, 0, ks[u], 2 * C + 1, (int)qs[b]);
+      }
+  }
+
+  // Moves the reference maxima where scores pass them by too much.
+  __device__ __forceinline__ void raise(const f4 (&s)[NQ][NS], float scale) {
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      float top = s[b][0][0];
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][u][i]);
+      top *= scale;
+      if (__any(top > m[b] + AT_SLACK)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m[b]);
+        const float f = __builtin_amdgcn_exp2f(m[b] - top);
+        m[b] = top;
+        l[b] *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[b][d] *= f;
+      }
+    }
+  }
+  // The scores become e^(score - m), p their bf16; the sums are kept up.
+  __device__ __forceinline__ void weigh(f4 (&s)[NQ][NS], bf16x8 (&p)[NQ][KB], float scale) {
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[b][u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][u][i], scale, -m[b]));
+          l[b] += s[b][u][i];
+          p[b][u / 2][4 * (u & 1) + i] = (bf16)s[b][u][i];
+        }
+  }
+
+  // O^T += V^T P^T from a buffer of operands.
+  __device__ __forceinline__ void values(const unsigned (*buf)[64][4], const bf16x8 (&p)[NQ][KB], int lane) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const bf16x8 v = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_t*>(&buf[kb * ND + d][lane][0]));
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[b][kb], o[b][d], 0, 0, 0);
+      }
+  }
+
+  // Masked tiles: keys that rows do not see; and NaN to the rows that see a value that reads as NaN.
+  __device__ __forceinline__ void hide(f4 (&s)[NQ][NS], int t0, int h) const {
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+#pragma unroll
+      for (int b = 0; b < NQ; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[b][u][i] = t0 + 16 * u + 4 * h + i <= last[b] ? s[b][u][i] : -__builtin_inff();
+  }
+  __device__ __forceinline__ void show_nan(const u64 (*nan)[4], int t0, int lane) {
+    const int h = lane >> 4;
+    if (!__any(nan[lane >> 2 & (AT_WAVES - 1)][lane & 3] != 0)) return;
+    unsigned hit[NQ];                            // bit c: in group 4 c + h, which holds all of the lane's channels of chunk c
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) hit[b] = 0;
+#pragma unroll 1
+    for (int j = 0; j < NS * NC * 16; ++j) {     // block and chunk, token 4 v + i
+      const int u = j / 16 / NC, v = j / 4 % 4, i = j % 4;
+      const unsigned one = (unsigned)(nan[j / 16][i] >> (16 * v + 4 * h)) & 1u;
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) hit[b] |= (t0 + 16 * u + 4 * v + i <= last[b] ? one : 0u) << (j / 16 % NC);
+    }
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        if (hit[b] >> (d / 8) & 1u) o[b][d] = f4(__builtin_nanf(""));
+  }
+};
+
+constexpr int prompt_waves(int D) { return 2; }   // a SIMD: what the registers and two workgroups' LDS allow
+
+template <int D>
+__global__ void __launch_bounds__(64 * AT_WAVES, prompt_waves(D)) prompt_kernel(AttnArgs a) {
+  using PR = Prompt<D>;
+  constexpr int KT = PR::KT, R = PR::R, NQ = PR::NQ, RING = PR::RING;
+  __shared__ typename PR::Shared sh;
+  const int lane = threadIdx.x & 63, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned raw0 = (unsigned)(size_t)(lds_void*)&sh.raw[0];
+  const int mine = 16 * (wave / PR::NC);         // the first of a tile's 16 tokens that this wave copies and decodes
+  Walk<R, KT> k(a);
+  clear_rest<bf16>(a, D);
+  const int64_t pb = kv_page_bytes(a.page, D);
+  while (k.next()) {
+    PR w;
+    const int* table = a.blocks + k.r * a.W;
+    const uint8_t* base = a.cache + (int64_t)k.head * pb;
+    const int full = min(k.kmin, k.kb), ka = k.ka, kb = k.kb;
+    bool bad = false;
+    Pages<1> page;
+    const auto copy = [&](int t0, int slot) {    // and looks up the page of the tile after
+      const uint8_t* p = base + page.at(a, 0, t0 + mine, pb, kv_sub_bytes(D), bad);
+      PR::copy(p, p + a.Hk * pb, raw0 + slot * (int)sizeof(typename PR::Raw), wave, lane);
+      page.look(a, table, t0 + KT + mine, kb - 1);
+    };
+    const auto stage = [&](int t0, int slot, int to) {
+      PR::stage_values(sh.raw[slot], sh.operands[to], sh.nans[to][wave], wave, t0 + mine, t0 + KT > full, kb, lane);
+    };
+    if (threadIdx.x == 0) sh.lost = 0;
+    if (ka < kb) {
+      page.look(a, table, ka + mine, kb - 1);
+#pragma unroll
+      for (int i = 0; i < RING - 1; ++i) copy(ka + i * KT, i);
+    }
+    w.begin(a, k.x, k.head, k.j * R + wave * 16 * NQ, k.G, lane);
+    if (ka < kb) {
+      wait_vmcnt<0>();
+      lds_barrier();                             // the first tiles are there
+      stage(ka, 0, 0);
+      lds_barrier();
+    }
+    int slot = 0, at = 0;                        // tile t0 is in raw[slot] and operands[at]
+    for (int t0 = ka; t0 < kb; t0 += KT, at ^= 1) {
+      const int after = slot + 1 == RING ? 0 : slot + 1;
+      const bool masked = t0 + KT > full;
+      f4 s[NQ][PR::NS];
+      bf16x8 p[NQ][PR::KB];
+      copy(t0 + (RING - 1) * KT, slot == 0 ? RING - 1 : slot - 1);
+      w.scores(sh.raw[slot], s, lane);
+      if (masked) w.hide(s, t0, h);
+      w.raise(s, a.scale);
+      w.weigh(s, p, a.scale);
+      stage(t0 + KT, after, at ^ 1);
+      w.values(sh.operands[at], p, lane);
+      if (masked) {                              // what P's first term leaves, for rows of few keys; NaNs
+        asm volatile("" : : : "memory");         // (not to be formed ahead of the branch)
+#pragma unroll
+        for (int b = 0; b < NQ; ++b)
+#pragma unroll
+          for (int u = 0; u < PR::NS; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int e = 4 * (u & 1) + i;
+              p[b][u / 2][e] = (bf16)(s[b][u][i] - (float)p[b][u / 2][e]);
+            }
+        w.values(sh.operands[at], p, lane);
+        w.show_nan(sh.nans[at], t0, lane);
+      }
+      wait_vmcnt<3 * (RING - 3)>();              // the tile after the next is there
+      lds_barrier();                             // for every wave; and its operands are written, this tile's read
+      slot = after;
+    }
+    wait_vmcnt<0>();                             // copies of tiles past the end
+    if (bad) sh.lost = 1;
+    __syncthreads();
+    const bool lost = sh.lost != 0;
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      w.l[b] += __shfl_xor(w.l[b], 16);
+      w.l[b] += __shfl_xor(w.l[b], 32);
+      if (lost) w.l[b] = __builtin_nanf("");
+    }
+    write_rows<bf16, D, NQ, R>(a, k, wave * 16 * NQ, w.o, w.m, w.l, lane);
+    __syncthreads();                             // everything of this piece has been read
+    k.done();
+  }
+  k.end();
 }
 
-// Joins the parts of each row group that several workgroups worked on: block (w, y) the rows 4 y .. 4 y + 3 of the one that
-// workgroup w began, a wave a row.
-template <typename T, int D, int R>
+// Joins the parts of a row group that several workgroups worked on: block (w, y) takes rows WAVES_A_ROW... of the group
+// that workgroup w began.  SPREAD: one row, its parts over the block's four waves (one long context leaves a few rows with
+// a hundred parts each: 262,144 tokens, 8 heads, 30 -> JOIN_US us); else a wave a row.
+template <typename T, int D, int R, bool SPREAD>
 __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
-  const int w = blockIdx.x, lane = threadIdx.x & 63, lrow = blockIdx.y * 4 + (threadIdx.x >> 6);
+  constexpr int PER = D / 64;
+  typedef float row_t __attribute__((ext_vector_type(PER)));
+  __shared__ row_t sums[SPREAD ? 3 : 1][64];
+  const int w = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lrow = SPREAD ? blockIdx.y : blockIdx.y * 4 + wave;
   const int4 rec = a.records[w];
   if (!rec.w) return;
   const int G = a.Hq / a.Hk;
@@ -615,54 +1034,75 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
   const int head = rec.y / x.groups, j = rec.y - head * x.groups;
   const int row = j * R + lrow, i = row / G, g = row - i * G;
   if (i >= x.qlen) return;
-  constexpr int PER = D / 64;
-  const auto at = [&](int v) { return a.part + ((int64_t)(2 * v + (v == w ? rec.w - 1 : 0)) * R + lrow) * (D + 4); };
-  float m = AT_LOWEST, l = 0.f, o[PER];
+  const int n = rec.z - w + 1;                   // parts: w's last piece, then the first ones of w + 1 .. rec.z
+  const auto part = [&](int v) {
+    return a.part + ((int64_t)(2 * (w + v) + (v == 0 ? rec.w - 1 : 0)) * R + lrow) * (D + 4);
+  };
+  float top = AT_LOWEST;
+  for (int v = lane; v < n; v += 64) top = fmaxf(top, part(v)[D]);
 #pragma unroll
-  for (int e = 0; e < PER; ++e) o[e] = 0.f;
-  for (int v = w; v <= rec.z; ++v) {
-    const float* p = at(v);
-    const float pm = p[D], pl = p[D + 1], top = fmaxf(m, pm);
-    const float f = __builtin_amdgcn_exp2f(m - top), g2 = __builtin_amdgcn_exp2f(pm - top);
-    m = top;
-    l = l * f + pl * g2;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) o[e] = o[e] * f + p[lane * PER + e] * g2;
+  for (int d = 32; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+  float l = 0.f;
+  row_t o = {};
+  for (int v0 = 0; v0 < n; v0 += 64) {
+    float f = 0.f;
+    if (v0 + lane < n) {
+      const float* p = part(v0 + lane);
+      f = __builtin_amdgcn_exp2f(p[D] - top);
+      l += p[D + 1] * f;
+    }
+    const int m = min(64, n - v0);
+#pragma unroll 8
+    for (int v = SPREAD ? wave : 0; v < m; v += SPREAD ? 4 : 1)
+      o += *reinterpret_cast<const row_t*>(part(v0 + v) + lane * PER) * __shfl(f, v);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* p = (T*)a.o + ((int64_t)(x.q0 + i) * a.Hq + head * G + g) * D + lane * PER;
 #pragma unroll
-  for (int e = 0; e < PER; ++e) p[e] = (T)(o[e] * inv);
+  for (int d = 32; d >= 1; d /= 2) l += __shfl_xor(l, d);
+  if constexpr (SPREAD) {
+    if (wave) sums[wave - 1][lane] = o;
+    __syncthreads();
+    if (wave) return;
+    for (int v = 0; v < 3; ++v) o += sums[v][lane];
+  }
+  o *= l == 0.f ? 0.f : 1.f / l;
+  T* p = (T*)a.o + ((int64_t)(x.q0 + i) * a.Hq + head * G + g) * D + lane * PER;
+  typedef T out_t __attribute__((ext_vector_type(PER)));
+  *reinterpret_cast<out_t*>(p) = __builtin_convertvector(o, out_t);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
-// Rows a wave takes and how the waves share the work, by the rows a request has on average: up to 16, and up to 32, the
-// waves split the keys (the chip is filled by keys alone); above, the rows.
+// Rows to a group, how the waves share the work, and the workgroups, by the rows that a request has on average: up to 16,
+// and up to 32, the waves split the keys (the chip is filled by keys alone); above, the rows.
 struct Shape {
-  int nq;
-  bool keys;
-  int rows() const { return 16 * nq * (keys ? 1 : AT_WAVES); }
+  int kind, rows, workers;                       // kind 0: 16 rows, keys split; 1: 32 rows, keys split; 2: rows split
 };
-static Shape shape_for(int64_t T, int64_t B, int64_t G) {
+static Shape shape_for(int64_t T, int64_t B, int64_t G, int64_t D, int32_t dtype) {
   const int64_t rows = (T + B - 1) / B * G;
-  if (rows <= 16) return {1, true};
-  if (rows <= 32) return {2, true};
-  return {2, false};
+  if (rows <= 16) return {0, 16, 256 * waves_for((int)D)};
+  if (rows <= 32) return {1, 32, 256};
+  if (dtype == MACAI_GDR_BF16 && D >= 128)
+    return {2, D == 256 ? Prompt<256>::R : Prompt<128>::R, 256 * prompt_waves((int)D)};
+  return {2, 128, 256};
 }
-static int workers_for(const Shape& s, int64_t D) { return 256 * (s.keys && s.nq == 1 ? waves_for((int)D) : 1); }
 
 template <typename T, int D>
 static void launch(const Shape& s, const AttnArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)a.workers), join((unsigned)a.workers, (unsigned)(s.rows() / 4));
-  if (s.keys && s.nq == 1) {
-    hipLaunchKernelGGL((attend_kernel<T, D, 1, true>), grid, dim3(64 * AT_WAVES), 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 16>), join, dim3(256), 0, st, a);
-  } else if (s.keys) {
-    hipLaunchKernelGGL((attend_kernel<T, D, 2, true>), grid, dim3(64 * AT_WAVES), 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 32>), join, dim3(256), 0, st, a);
+  // the rows of a group that can exist: without starts a request has one query
+  const int rows = s.kind < 2 && !a.starts ? (int)std::min<int64_t>(a.Hq / a.Hk, s.rows) : s.rows;
+  const dim3 grid((unsigned)a.workers), join((unsigned)a.workers, (unsigned)(s.kind < 2 ? rows : rows / 4));
+  const dim3 threads(64 * AT_WAVES);
+  if (s.kind == 0) {
+    hipLaunchKernelGGL((attend_kernel<T, D, 1, true>), grid, threads, 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, 16, true>), join, dim3(256), 0, st, a);
+  } else if (s.kind == 1) {
+    hipLaunchKernelGGL((attend_kernel<T, D, 2, true>), grid, threads, 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, 32, true>), join, dim3(256), 0, st, a);
+  } else if constexpr (std::is_same<T, bf16>::value && D >= 128) {
+    hipLaunchKernelGGL((prompt_kernel<D>), grid, threads, 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, Prompt<D>::R, false>), join, dim3(256), 0, st, a);
   } else {
-    hipLaunchKernelGGL((attend_kernel<T, D, 2, false>), grid, dim3(64 * AT_WAVES), 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 128>), join, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attend_kernel<T, D, 2, false>), grid, threads, 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, 128, false>), join, dim3(256), 0, st, a);
   }
 }
 
@@ -677,11 +1117,10 @@ static void launch_width(int64_t D, const Shape& s, const AttnArgs& a, hipStream
 
 extern "C" {
 
-int64_t macai_gdr_kv4_attention_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D) {
+int64_t macai_gdr_kv4_attention_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int32_t dtype) {
   if (T < 1 || B < 1 || Hk < 1 || Hq < Hk || D < 1) return 0;
-  const gdr::Shape s = gdr::shape_for(T, B, Hq / Hk);
-  const int64_t n = gdr::workers_for(s, D);
-  return n * (int64_t)sizeof(int4) + 2 * n * s.rows() * (D + 4) * (int64_t)sizeof(float);
+  const gdr::Shape s = gdr::shape_for(T, B, Hq / Hk, D, dtype);
+  return s.workers * (int64_t)(sizeof(int4) + 2 * s.rows * (D + 4) * sizeof(float));
 }
 
 int macai_gdr_kv4_attention(const void* q, const uint8_t* cache, const int32_t* blocks, const int32_t* lens,
@@ -708,9 +1147,9 @@ int macai_gdr_kv4_attention(const void* q, const uint8_t* cache, const int32_t* 
     if (!aligned16(p)) return fail(MACAI_GDR_EINVAL, "%s: pointers must be 16-byte aligned", what);
   const int64_t v = dtype == MACAI_GDR_F32 ? 4 : 8;
   if (q_row % v || q_head % v) return fail(MACAI_GDR_EINVAL, "%s: strides must keep 16-byte alignment", what);
-  const gdr::Shape s = gdr::shape_for(T, B, Hq / Hk);
+  const gdr::Shape s = gdr::shape_for(T, B, Hq / Hk, D, dtype);
   gdr::AttnArgs a{q, o, cache, blocks, lens, starts, nullptr, nullptr, q_row, q_head, T, B, W, pages, (int)Hq, (int)Hk,
-                  (int)page, __builtin_ctzll((unsigned long long)page), gdr::workers_for(s, D), scale * 1.44269504088896341f};
+                  (int)page, __builtin_ctzll((unsigned long long)page), s.workers, scale * 1.44269504088896341f};
   a.records = (int4*)workspace;
   a.part = (float*)((char*)workspace + a.workers * sizeof(int4));
   hipStream_t st = (hipStream_t)stream;

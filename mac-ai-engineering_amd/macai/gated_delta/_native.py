@@ -49,7 +49,7 @@ SIGNATURES = {
     "macai_gdr_kv4_plan": [_p] * 10 + [_i64] * 5 + [_p],
     "macai_gdr_kv4_append": [_p] * 8 + [_i64] * 14 + [_i32] * 3 + [_p],
     "macai_gdr_kv4_read": [_p] * 4 + [_i64] * 5 + [_i32, _p],
-    "macai_gdr_kv4_attention_workspace": [_i64] * 5,
+    "macai_gdr_kv4_attention_workspace": [_i64] * 5 + [_i32],
     "macai_gdr_kv4_attention": [_p] * 7 + [_i64] * 10 + [_f, _i32, _p],
     "macai_gdr_probe_stream": [_i32, _p, _p, _i64, _i32, _p],
     "macai_gdr_probe_mfma": [_i32, _i32, _p, _i32, _p],

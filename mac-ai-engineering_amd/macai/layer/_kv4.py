@@ -191,9 +191,10 @@ def kv4_attention(q, cache, blocks, lens, starts=None, scale: float = None):
         return torch.zeros(T, Hq, D, dtype=q.dtype, device=q.device)
     o = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
     q, q_row, q_head = _rows(q, "q")
-    work = torch.empty(N.lib().macai_gdr_kv4_attention_workspace(T, B, Hq, Hk, D), dtype=torch.uint8, device=q.device)
+    code = N.dtype_code(q.dtype, True)
+    work = torch.empty(N.lib().macai_gdr_kv4_attention_workspace(T, B, Hq, Hk, D, code), dtype=torch.uint8, device=q.device)
     with _on(q.device):
         N.call("macai_gdr_kv4_attention", q.data_ptr(), cache.data_ptr(), blocks.data_ptr(), lens.data_ptr(), N.ptr(starts),
                o.data_ptr(), work.data_ptr(), T, B, W, cache.shape[0], page, Hq, Hk, D, q_row, q_head,
-               D ** -0.5 if scale is None else float(scale), N.dtype_code(q.dtype, True), N.stream_of(q))
+               D ** -0.5 if scale is None else float(scale), code, N.stream_of(q))
     return o

@@ -153,5 +153,5 @@ def test_abi_refusals(name, args, bad, code, why):
 
 def test_workspace_sizes():
     f = N.lib().macai_gdr_kv4_attention_workspace
-    assert f(0, 1, 8, 2, 128) == 0 and f(1, 1, 1, 2, 128) == 0
-    assert f(64, 64, 16, 2, 256) > 0 and f(4096, 4, 16, 2, 256) > 0
+    assert f(0, 1, 8, 2, 128, 1) == 0 and f(1, 1, 1, 2, 128, 1) == 0
+    assert f(64, 64, 16, 2, 256, 1) > 0 and f(4096, 4, 16, 2, 256, 0) > 0
