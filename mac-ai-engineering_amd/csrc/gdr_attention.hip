@@ -257,9 +257,12 @@ __device__ __forceinline__ void clear_rest(const AttnArgs& a, int D) {
 template <int NS>
 struct Pages {
   int id[NS];
+  // (a scalar load: as a vector load its wait would be one for every copy in flight)
   __device__ __forceinline__ void look(const AttnArgs& a, const int* table, int t0, int last) {
+    typedef const __attribute__((address_space(4))) int scalar_int;
+    scalar_int* t = (scalar_int*)(size_t)table;
 #pragma unroll
-    for (int u = 0; u < NS; ++u) id[u] = table[min(t0 + 16 * u, last) >> a.page_shift];
+    for (int u = 0; u < NS; ++u) id[u] = t[min(t0 + 16 * u, last) >> a.page_shift];
   }
   // the byte offset of block u of these, of the tokens from t0 on, from a head's keys on; bad: a number out of range
   __device__ __forceinline__ int64_t at(const AttnArgs& a, int u, int t0, int64_t pb, int sub, bool& bad) const {
