@@ -525,6 +525,14 @@ __device__ __forceinline__ int channel(int d, int h, int i) {
   return d / RUN * (16 * RUN) + (4 * h + i) * RUN + d % RUN;
 }
 
+// Parts of a row group's results lie as a wave holds them, [R / 16 blocks of rows][D / 16 tiles][64 lanes] of f4 (rows apart,
+// a store was 64 lines of 16 bytes: 5 of the 24 us of the prompts' join and most of what a split piece took to end), then
+// R maxima and R sums.  A workgroup has two: its first piece's and its last's.
+template <int R, int D>
+__device__ __forceinline__ float* part_of(const AttnArgs& a, int w, bool opening) {
+  return a.part + (int64_t)(2 * w + (opening ? 0 : 1)) * R * (D + 4);
+}
+
 // A wave's 16 NQ rows from lrow0 of the row group on: whole results to o, parts to the workspace.
 template <typename T, int D, int NQ, int R, typename W>
 __device__ __forceinline__ void write_rows(const AttnArgs& a, const W& k, int lrow0, const f4 (&o)[NQ][D / 16],
@@ -548,17 +556,12 @@ __device__ __forceinline__ void write_rows(const AttnArgs& a, const W& k, int lr
           for (int f = 0; f < RUN; ++f) v[f] = (T)(o[b][c * RUN + f][e] * inv);
           *reinterpret_cast<run_t*>(p + channel<D>(c * RUN, h, e)) = v;
         }
-    } else {
-      float* p = a.part + ((int64_t)(2 * k.w + (k.opening ? 0 : 1)) * R + lrow) * (D + 4);
+    } else if (i < k.x.qlen) {
+      float* p = part_of<R, D>(a, k.w, k.opening);
+      f4* q = reinterpret_cast<f4*>(p) + (lrow / 16) * ND * 64 + lane;
 #pragma unroll
-      for (int c = 0; c < ND / RUN; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int f = 0; f < RUN; f += 4)
-            *reinterpret_cast<f4*>(p + channel<D>(c * RUN, h, e) + f) =
-                f4{o[b][c * RUN + f][e], o[b][c * RUN + f + 1][e], o[b][c * RUN + f + 2][e], o[b][c * RUN + f + 3][e]};
-      if (h == 0) p[D] = m[b], p[D + 1] = l[b];
+      for (int d = 0; d < ND; ++d) q[d * 64] = o[b][d];
+      if (h == 0) p[R * D + lrow] = m[b], p[R * D + R + lrow] = l[b];
     }
   }
 }
@@ -888,16 +891,28 @@ struct Prompt {
         }
   }
 
-  // O^T += V^T P^T from a buffer of operands.
+  // O^T += V^T P^T from a buffer of operands, four fragments in flight (with two, each pair of reads waited out its latency:
+  // FRAG_US).
   __device__ __forceinline__ void values(const unsigned (*buf)[64][4], const bf16x8 (&p)[NQ][KB], int lane) {
+    constexpr int N = KB * ND, AHEAD = D == 256 ? 2 : 4;
+    u32x4_t v[AHEAD];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int i = 0; i < AHEAD; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(&buf[i][lane][0]);
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const bf16x8 v = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_t*>(&buf[kb * ND + d][lane][0]));
+    for (int i = 0; i < N; ++i) {
+      const bf16x8 f = __builtin_bit_cast(bf16x8, v[i % AHEAD]);
 #pragma unroll
-        for (int b = 0; b < NQ; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[b][kb], o[b][d], 0, 0, 0);
-      }
+      for (int b = 0; b < NQ; ++b)
+        o[b][i % ND] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, p[b][i / ND], o[b][i % ND], 0, 0, 0);
+      if (i + AHEAD < N) v[i % AHEAD] = *reinterpret_cast<const u32x4_t*>(&buf[i + AHEAD][lane][0]);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 1);
+#pragma unroll
+    for (int i = 0; i + AHEAD < N; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, NQ, 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, NQ * AHEAD, 1);
   }
 
   // Masked tiles: keys that rows do not see; and NaN to the rows that see a value that reads as NaN.
@@ -1020,57 +1035,72 @@ __global__ void __launch_bounds__(64 * AT_WAVES, prompt_waves(D)) prompt_kernel(
   k.end();
 }
 
-// Joins the parts of a row group that several workgroups worked on: block (w, y) takes rows WAVES_A_ROW... of the group
-// that workgroup w began.  SPREAD: one row, its parts over the block's four waves (one long context leaves a few rows with
-// a hundred parts each: 262,144 tokens, 8 heads, 30 -> JOIN_US us); else a wave a row.
-template <typename T, int D, int R, bool SPREAD>
-__global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
-  constexpr int PER = D / 64;
-  typedef float row_t __attribute__((ext_vector_type(PER)));
-  __shared__ row_t sums[SPREAD ? 3 : 1][64];
-  const int w = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int lrow = SPREAD ? blockIdx.y : blockIdx.y * 4 + wave;
-  const int4 rec = a.records[w];
+// Joins the parts of a row group that several workgroups worked on: block (w, y) takes 16 rows and one chunk of channels
+// (RUN output tiles) of the group that workgroup w began, its parts shared by WAVES waves (one long context leaves a few
+// rows with a hundred parts each).
+template <typename T, int D, int R, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) join_kernel(AttnArgs a) {
+  constexpr int RUN = D < 128 ? D / 16 : 8, ND = D / 16;
+  typedef T run_t __attribute__((ext_vector_type(RUN)));
+  __shared__ f4 sums[WAVES > 1 ? WAVES - 1 : 1][RUN][64];
+  __shared__ float totals[WAVES][16];
+  const int4 rec = a.records[blockIdx.x];
   if (!rec.w) return;
+  const int w = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 4, n = lane & 15;
+  const int block = blockIdx.y / (ND / RUN), chunk = blockIdx.y % (ND / RUN), lrow = block * 16 + n;
   const int G = a.Hq / a.Hk;
   const Req x = request<R>(a, rec.x, G);
   const int head = rec.y / x.groups, j = rec.y - head * x.groups;
+  if ((j * R + block * 16) / G >= x.qlen) return;   // none of these rows exist
   const int row = j * R + lrow, i = row / G, g = row - i * G;
-  if (i >= x.qlen) return;
-  const int n = rec.z - w + 1;                   // parts: w's last piece, then the first ones of w + 1 .. rec.z
-  const auto part = [&](int v) {
-    return a.part + ((int64_t)(2 * (w + v) + (v == 0 ? rec.w - 1 : 0)) * R + lrow) * (D + 4);
-  };
+  const bool there = i < x.qlen;
+  const int parts = rec.z - w + 1;               // w's last piece, then the first ones of w + 1 .. rec.z
+  const auto part = [&](int v) { return part_of<R, D>(a, w + v, v ? true : rec.w == 1); };
+  // the rows' reference maxima over all parts: lane quarters take every fourth
   float top = AT_LOWEST;
-  for (int v = lane; v < n; v += 64) top = fmaxf(top, part(v)[D]);
-#pragma unroll
-  for (int d = 32; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (there)
+    for (int v = h; v < parts; v += 4) top = fmaxf(top, part(v)[R * D + lrow]);
+  top = fmaxf(top, __shfl_xor(top, 16));
+  top = fmaxf(top, __shfl_xor(top, 32));
   float l = 0.f;
-  row_t o = {};
-  for (int v0 = 0; v0 < n; v0 += 64) {
-    float f = 0.f;
-    if (v0 + lane < n) {
-      const float* p = part(v0 + lane);
-      f = __builtin_amdgcn_exp2f(p[D] - top);
-      l += p[D + 1] * f;
-    }
-    const int m = min(64, n - v0);
-#pragma unroll 8
-    for (int v = SPREAD ? wave : 0; v < m; v += SPREAD ? 4 : 1)
-      o += *reinterpret_cast<const row_t*>(part(v0 + v) + lane * PER) * __shfl(f, v);
-  }
+  f4 o[RUN];
 #pragma unroll
-  for (int d = 32; d >= 1; d /= 2) l += __shfl_xor(l, d);
-  if constexpr (SPREAD) {
-    if (wave) sums[wave - 1][lane] = o;
+  for (int e = 0; e < RUN; ++e) o[e] = f4{0.f, 0.f, 0.f, 0.f};
+  if (there) {
+#pragma unroll 2
+    for (int v = wave; v < parts; v += WAVES) {
+      const float* p = part(v);
+      const f4* q = reinterpret_cast<const f4*>(p) + (block * ND + chunk * RUN) * 64 + lane;
+      const float f = __builtin_amdgcn_exp2f(p[R * D + lrow] - top);
+      l += p[R * D + R + lrow] * f;
+#pragma unroll
+      for (int e = 0; e < RUN; ++e) o[e] += q[e * 64] * f;
+    }
+  }
+  if constexpr (WAVES > 1) {
+    if (h == 0) totals[wave][n] = l;
+    if (wave) {
+#pragma unroll
+      for (int e = 0; e < RUN; ++e) sums[wave - 1][e][lane] = o[e];
+    }
     __syncthreads();
     if (wave) return;
-    for (int v = 0; v < 3; ++v) o += sums[v][lane];
+    l = 0.f;
+    for (int v = 0; v < WAVES; ++v) l += totals[v][n];
+    for (int v = 0; v < WAVES - 1; ++v)
+#pragma unroll
+      for (int e = 0; e < RUN; ++e) o[e] += sums[v][e][lane];
   }
-  o *= l == 0.f ? 0.f : 1.f / l;
-  T* p = (T*)a.o + ((int64_t)(x.q0 + i) * a.Hq + head * G + g) * D + lane * PER;
-  typedef T out_t __attribute__((ext_vector_type(PER)));
-  *reinterpret_cast<out_t*>(p) = __builtin_convertvector(o, out_t);
+  if (!there) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* p = (T*)a.o + ((int64_t)(x.q0 + i) * a.Hq + head * G + g) * D;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    run_t v;
+#pragma unroll
+    for (int f = 0; f < RUN; ++f) v[f] = (T)(o[f][e] * inv);
+    *reinterpret_cast<run_t*>(p + channel<D>(chunk * RUN, h, e)) = v;
+  }
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
@@ -1090,22 +1120,20 @@ static Shape shape_for(int64_t T, int64_t B, int64_t G, int64_t D, int32_t dtype
 
 template <typename T, int D>
 static void launch(const Shape& s, const AttnArgs& a, hipStream_t st) {
-  // the rows of a group that can exist: without starts a request has one query
-  const int rows = s.kind < 2 && !a.starts ? (int)std::min<int64_t>(a.Hq / a.Hk, s.rows) : s.rows;
-  const dim3 grid((unsigned)a.workers), join((unsigned)a.workers, (unsigned)(s.kind < 2 ? rows : rows / 4));
-  const dim3 threads(64 * AT_WAVES);
+  constexpr int CHUNKS = D < 128 ? 1 : D / 128;
+  const dim3 grid((unsigned)a.workers), threads(64 * AT_WAVES), join((unsigned)a.workers, (unsigned)(s.rows / 16 * CHUNKS));
   if (s.kind == 0) {
     hipLaunchKernelGGL((attend_kernel<T, D, 1, true>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 16, true>), join, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, 16, 8>), join, dim3(512), 0, st, a);
   } else if (s.kind == 1) {
     hipLaunchKernelGGL((attend_kernel<T, D, 2, true>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 32, true>), join, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, 32, 4>), join, dim3(256), 0, st, a);
   } else if constexpr (std::is_same<T, bf16>::value && D >= 128) {
     hipLaunchKernelGGL((prompt_kernel<D>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, Prompt<D>::R, false>), join, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, Prompt<D>::R, 1>), join, dim3(64), 0, st, a);
   } else {
     hipLaunchKernelGGL((attend_kernel<T, D, 2, false>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 128, false>), join, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, 128, 1>), join, dim3(64), 0, st, a);
   }
 }
 
