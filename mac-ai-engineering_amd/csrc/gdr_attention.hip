@@ -40,7 +40,6 @@ typedef unsigned long long u64;
 
 constexpr int AT_WAVES = 4;
 constexpr float AT_LOWEST = -3.402823466e38f;    // a reference maximum below every score; exp2(-inf - it) is 0
-constexpr int AT_BEGIN = 128;
 constexpr float AT_SLACK = 8.f;                  // how far (log2) scores may pass the reference maximum
 
 struct AttnArgs {
@@ -57,20 +56,22 @@ struct AttnArgs {
 };
 
 // A request as the split sees it.  Costs are in tokens: a row group j of a head costs base + (j + 1) per, the keys its
-// last row sees, rounded up where G does not divide R (a few tokens too many, never too few), and AT_BEGIN for what a row
-// group takes besides (its queries, the first loads, its results; without it workgroups with many short row groups ended
-// last: prompts, half the waves' time).
+// last row sees, rounded up where G does not divide R (a few tokens too many, never too few), and `begin` for what a row
+// group takes besides (its queries, the first loads, its results: as long as 128 tokens where keys stream, 13 us or 256
+// tokens in chunks of prompts; without it workgroups with many short row groups ended last).
 struct Req {
   int q0, qlen, len, base;                       // first query row, queries, tokens, tokens before the queries
   int groups;                                    // row groups a head
+  int begin;
   __device__ __forceinline__ int64_t cost(int64_t j, int per) const {
-    return j * (base + AT_BEGIN) + (int64_t)per * j * (j + 1) / 2;
+    return j * (base + begin) + (int64_t)per * j * (j + 1) / 2;
   }
 };
 
 template <int R>
 __device__ __forceinline__ Req request(const AttnArgs& a, int64_t r, int G) {
   Req x;
+  x.begin = R <= 32 ? 128 : 256;
   const int64_t most = a.W * a.page;
   x.len = (int)min((int64_t)max(a.lens[r], 0), most);
   if (a.starts) {
@@ -226,8 +227,8 @@ struct Walk {
       // the keys: at most the last row's, both ends of a split rounded to whole steps
       const int rows = min(R, x.qlen * G - j * R), all = x.len - x.qlen + (j * R + rows - 1) / G + 1;
       kmin = x.len - x.qlen + (j * R) / G + 1;
-      ka = max((int)(x0 - u0) - AT_BEGIN, 0) / STEP * STEP;
-      kb = min(all, stop == u1 ? all : max((int)(stop - u0) - AT_BEGIN, 0) / STEP * STEP);
+      ka = max((int)(x0 - u0) - x.begin, 0) / STEP * STEP;
+      kb = min(all, stop == u1 ? all : max((int)(stop - u0) - x.begin, 0) / STEP * STEP);
       return true;
     }
     return false;
@@ -700,35 +701,36 @@ struct Prompt {
   float m[NQ], l[NQ];
   int last[NQ];
 
+  // Channels 128 C + 64 part + 16 h + 0..15 of a row, as loaded, to its two terms and scales.
   template <int C>
-  __device__ __forceinline__ void begin_chunk(const bf16* p, int b, bool there, int lane) {
+  __device__ __forceinline__ void split(const u32x4_t (&raw)[2][2], int b, bool there, int lane) {
     const int h = lane >> 4;
-    float v[2][8], w[2][8];
-    float top[2] = {0.f, 0.f};
     int e[2];
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-      load_f8(p + C * 128 + part * 64 + 16 * h, v[part]);
-      load_f8(p + C * 128 + part * 64 + 16 * h + 8, w[part]);
+      float x[16];
       unsigned bits = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (!there) v[part][i] = w[part][i] = 0.f;
-        bits = max(bits, max(__float_as_uint(v[part][i]) & 0x7FFFFFFFu, __float_as_uint(w[part][i]) & 0x7FFFFFFFu));
+        const unsigned w = there ? raw[part][i / 4][i % 4] : 0u;
+        x[2 * i] = __uint_as_float(w << 16);
+        x[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
+        bits = max(bits, max(w << 16 & 0x7FFFFFFFu, w & 0x7FFF0000u));
       }
       bits = max(bits, (unsigned)__shfl_xor((int)bits, 16));       // the group's other half
       e[part] = bits >= 0x7F800000u ? 255 : max((int)(bits >> 23) - 7, 8);
       const float down = __uint_as_float((unsigned)(254 - min(e[part], 253)) << 23);   // 2^(127 - e): values up to 256
 #pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= down;
+#pragma unroll
       for (int i = 0; i < 4; ++i) {              // 4 bytes from 4 channels
-        const float x[4] = {(i < 2 ? v : w)[part][4 * (i & 1)] * down, (i < 2 ? v : w)[part][4 * (i & 1) + 1] * down,
-                            (i < 2 ? v : w)[part][4 * (i & 1) + 2] * down, (i < 2 ? v : w)[part][4 * (i & 1) + 3] * down};
-        int hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-        hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], hi, true);
-        int lo = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - __builtin_amdgcn_cvt_f32_fp8(hi, 0)) * 16.f,
-                                                 (x[1] - __builtin_amdgcn_cvt_f32_fp8(hi, 1)) * 16.f, 0, false);
-        lo = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - __builtin_amdgcn_cvt_f32_fp8(hi, 2)) * 16.f,
-                                             (x[3] - __builtin_amdgcn_cvt_f32_fp8(hi, 3)) * 16.f, lo, true);
+        const float* y = x + 4 * i;
+        int hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], hi, true);
+        int lo = __builtin_amdgcn_cvt_pk_fp8_f32((y[0] - __builtin_amdgcn_cvt_f32_fp8(hi, 0)) * 16.f,
+                                                 (y[1] - __builtin_amdgcn_cvt_f32_fp8(hi, 1)) * 16.f, 0, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32((y[2] - __builtin_amdgcn_cvt_f32_fp8(hi, 2)) * 16.f,
+                                             (y[3] - __builtin_amdgcn_cvt_f32_fp8(hi, 3)) * 16.f, lo, true);
         q[b][C][0][part * 4 + i] = hi;
         q[b][C][1][part * 4 + i] = lo;
       }
@@ -739,16 +741,28 @@ struct Prompt {
   }
 
   __device__ __forceinline__ void begin(const AttnArgs& a, const Req& x, int head, int row0, int G, int lane) {
-    const int n = lane & 15;
+    const int h = lane >> 4, n = lane & 15;
+    u32x4_t raw[NQ][NC][2][2];                   // all loads before the first use
+    bool there[NQ];
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
       const int row = row0 + b * 16 + n, i = row / G, g = row - i * G;
-      const bool there = i < x.qlen;
-      last[b] = there ? x.len - x.qlen + i : -1;
-      const bf16* p = (const bf16*)a.q + (x.q0 + (there ? i : 0)) * a.q_row + (int64_t)(head * G + g) * a.q_head;
+      there[b] = i < x.qlen;
+      last[b] = there[b] ? x.len - x.qlen + i : -1;
+      const bf16* p = (const bf16*)a.q + (x.q0 + (there[b] ? i : 0)) * a.q_row + (int64_t)(head * G + g) * a.q_head;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int i2 = 0; i2 < 2; ++i2)
+            raw[b][c][part][i2] = *reinterpret_cast<const u32x4_t*>(p + c * 128 + part * 64 + 16 * h + 8 * i2);
+    }
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
       qs[b] = 0;
-      begin_chunk<0>(p, b, there, lane);
-      if constexpr (NC == 2) begin_chunk<1>(p, b, there, lane);
+      split<0>(raw[b][0], b, there[b], lane);
+      if constexpr (NC == 2) split<NC - 1>(raw[b][NC - 1], b, there[b], lane);
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[b][d] = f4{0.f, 0.f, 0.f, 0.f};
       m[b] = AT_LOWEST;
@@ -1035,72 +1049,138 @@ __global__ void __launch_bounds__(64 * AT_WAVES, prompt_waves(D)) prompt_kernel(
   k.end();
 }
 
-// Joins the parts of a row group that several workgroups worked on: block (w, y) takes 16 rows and one chunk of channels
-// (RUN output tiles) of the group that workgroup w began, its parts shared by WAVES waves (one long context leaves a few
-// rows with a hundred parts each).
-template <typename T, int D, int R, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) join_kernel(AttnArgs a) {
-  constexpr int RUN = D < 128 ? D / 16 : 8, ND = D / 16;
+// ---- joining the parts of row groups that several workgroups worked on ---------------------------------------------
+// Block (w, y) takes 16 rows and one chunk of channels (RUN output tiles) of the group that workgroup w began.
+template <typename T, int D, int R>
+struct Join {
+  static constexpr int RUN = D < 128 ? D / 16 : 8, ND = D / 16;
   typedef T run_t __attribute__((ext_vector_type(RUN)));
-  __shared__ f4 sums[WAVES > 1 ? WAVES - 1 : 1][RUN][64];
-  __shared__ float totals[WAVES][16];
-  const int4 rec = a.records[blockIdx.x];
-  if (!rec.w) return;
-  const int w = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 4, n = lane & 15;
-  const int block = blockIdx.y / (ND / RUN), chunk = blockIdx.y % (ND / RUN), lrow = block * 16 + n;
-  const int G = a.Hq / a.Hk;
-  const Req x = request<R>(a, rec.x, G);
-  const int head = rec.y / x.groups, j = rec.y - head * x.groups;
-  if ((j * R + block * 16) / G >= x.qlen) return;   // none of these rows exist
-  const int row = j * R + lrow, i = row / G, g = row - i * G;
-  const bool there = i < x.qlen;
-  const int parts = rec.z - w + 1;               // w's last piece, then the first ones of w + 1 .. rec.z
-  const auto part = [&](int v) { return part_of<R, D>(a, w + v, v ? true : rec.w == 1); };
-  // the rows' reference maxima over all parts: lane quarters take every fourth
-  float top = AT_LOWEST;
-  if (there)
-    for (int v = h; v < parts; v += 4) top = fmaxf(top, part(v)[R * D + lrow]);
-  top = fmaxf(top, __shfl_xor(top, 16));
-  top = fmaxf(top, __shfl_xor(top, 32));
-  float l = 0.f;
-  f4 o[RUN];
-#pragma unroll
-  for (int e = 0; e < RUN; ++e) o[e] = f4{0.f, 0.f, 0.f, 0.f};
-  if (there) {
-#pragma unroll 2
-    for (int v = wave; v < parts; v += WAVES) {
-      const float* p = part(v);
-      const f4* q = reinterpret_cast<const f4*>(p) + (block * ND + chunk * RUN) * 64 + lane;
-      const float f = __builtin_amdgcn_exp2f(p[R * D + lrow] - top);
-      l += p[R * D + R + lrow] * f;
-#pragma unroll
-      for (int e = 0; e < RUN; ++e) o[e] += q[e * 64] * f;
-    }
+  int parts, chunk, lrow;                        // the group's parts; the lane's row
+  int64_t out;                                   // where its results go
+  bool some, there;                              // whether any of the 16 rows exist, and the lane's
+  int w, opening;
+
+  __device__ __forceinline__ Join(const AttnArgs& a, const int4& rec, int n) {
+    w = blockIdx.x;
+    const int block = blockIdx.y / (ND / RUN), G = a.Hq / a.Hk;
+    chunk = blockIdx.y % (ND / RUN);
+    lrow = block * 16 + n;
+    const Req x = request<R>(a, rec.x, G);
+    const int head = rec.y / x.groups, j = rec.y - head * x.groups, row = j * R + lrow, i = row / G;
+    some = (j * R + block * 16) / G < x.qlen;
+    there = i < x.qlen;
+    out = ((int64_t)(x.q0 + i) * a.Hq + head * G + row - i * G) * D;
+    parts = rec.z - w + 1;                       // w's last piece, then the first ones of w + 1 .. rec.z
+    opening = rec.w == 1;
   }
-  if constexpr (WAVES > 1) {
-    if (h == 0) totals[wave][n] = l;
-    if (wave) {
-#pragma unroll
-      for (int e = 0; e < RUN; ++e) sums[wave - 1][e][lane] = o[e];
-    }
-    __syncthreads();
-    if (wave) return;
-    l = 0.f;
-    for (int v = 0; v < WAVES; ++v) l += totals[v][n];
-    for (int v = 0; v < WAVES - 1; ++v)
-#pragma unroll
-      for (int e = 0; e < RUN; ++e) o[e] += sums[v][e][lane];
+  __device__ __forceinline__ const float* part(const AttnArgs& a, int v) const {
+    return part_of<R, D>(a, w + v, v ? true : opening);
   }
-  if (!there) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* p = (T*)a.o + ((int64_t)(x.q0 + i) * a.Hq + head * G + g) * D;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  __device__ __forceinline__ const f4* tiles(const AttnArgs& a, int v, int lane) const {
+    return reinterpret_cast<const f4*>(part(a, v)) + (lrow / 16 * ND + chunk * RUN) * 64 + lane;
+  }
+  // element e of the lane's RUN tiles, times inv
+  __device__ __forceinline__ void store(const AttnArgs& a, const float (&x)[RUN], float inv, int e, int h) const {
     run_t v;
 #pragma unroll
-    for (int f = 0; f < RUN; ++f) v[f] = (T)(o[f][e] * inv);
-    *reinterpret_cast<run_t*>(p + channel<D>(chunk * RUN, h, e)) = v;
+    for (int f = 0; f < RUN; ++f) v[f] = (T)(x[f] * inv);
+    *reinterpret_cast<run_t*>((T*)a.o + out + channel<D>(chunk * RUN, h, e)) = v;
   }
+};
+
+// Few parts (row groups of many rows, a wave a block).
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(64) join_kernel(AttnArgs a) {
+  using JT = Join<T, D, R>;
+  const int4 rec = a.records[blockIdx.x];
+  if (!rec.w) return;
+  const int lane = threadIdx.x, h = lane >> 4;
+  const JT j(a, rec, lane & 15);
+  if (!j.there) return;
+  float top = AT_LOWEST, l = 0.f;
+  for (int v = 0; v < j.parts; ++v) top = fmaxf(top, j.part(a, v)[R * D + j.lrow]);
+  f4 o[JT::RUN];
+#pragma unroll
+  for (int e = 0; e < JT::RUN; ++e) o[e] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int v = 0; v < j.parts; ++v) {
+    const float* p = j.part(a, v);
+    const f4* q = j.tiles(a, v, lane);
+    const float f = __builtin_amdgcn_exp2f(p[R * D + j.lrow] - top);
+    l += p[R * D + R + j.lrow] * f;
+#pragma unroll
+    for (int e = 0; e < JT::RUN; ++e) o[e] += q[e * 64] * f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float x[JT::RUN];
+#pragma unroll
+    for (int f = 0; f < JT::RUN; ++f) x[f] = o[f][e];
+    j.store(a, x, inv, e, h);
+  }
+}
+
+// Many parts: one long context leaves a few rows with a hundred of them, and what counts is how many loads are in flight.
+// All threads take the maxima and sums, a part to 16 of them; then each wave one part in WAVES / PAIRS of two tiles.
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(512) join_many_kernel(AttnArgs a) {
+  using JT = Join<T, D, R>;
+  constexpr int WAVES = 8, PAIRS = JT::RUN / 2, SPREAD = WAVES / PAIRS, SLOTS = 32, CHUNK = 128;
+  __shared__ float weight[CHUNK][16], tops[SLOTS][16], totals[SLOTS][16];
+  __shared__ f4 sums[SPREAD][JT::RUN][64];
+  const int4 rec = a.records[blockIdx.x];
+  if (!rec.w) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 4, n = lane & 15, slot = threadIdx.x >> 4;
+  const JT j(a, rec, n);
+  if (!j.some) return;
+  float top = AT_LOWEST, l = 0.f;
+  if (j.there) {
+#pragma unroll 4
+    for (int v = slot; v < j.parts; v += SLOTS) top = fmaxf(top, j.part(a, v)[R * D + j.lrow]);
+  }
+  tops[slot][n] = top;
+  __syncthreads();
+  for (int v = 0; v < SLOTS; ++v) top = fmaxf(top, tops[v][n]);
+  const int pair = wave % PAIRS, first = wave / PAIRS;
+  f4 o[2] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
+  for (int v0 = 0; v0 < j.parts; v0 += CHUNK) {
+    const int m = min(CHUNK, j.parts - v0);
+    __syncthreads();                             // the weights before these have been read
+    for (int v = slot; v < m; v += SLOTS) {
+      float f = 0.f;
+      if (j.there) {
+        const float* p = j.part(a, v0 + v);
+        f = __builtin_amdgcn_exp2f(p[R * D + j.lrow] - top);
+        l += p[R * D + R + j.lrow] * f;
+      }
+      weight[v][n] = f;
+    }
+    __syncthreads();
+    if (j.there) {
+#pragma unroll 8
+      for (int v = first; v < m; v += SPREAD) {
+        const f4* q = j.tiles(a, v0 + v, lane) + pair * 2 * 64;
+        const float f = weight[v][n];
+        o[0] += q[0] * f;
+        o[1] += q[64] * f;
+      }
+    }
+  }
+  totals[slot][n] = l;
+  sums[first][pair * 2][lane] = o[0];
+  sums[first][pair * 2 + 1][lane] = o[1];
+  __syncthreads();
+  if (wave >= 4 || !j.there) return;
+  l = 0.f;
+  for (int v = 0; v < SLOTS; ++v) l += totals[v][n];
+  float x[JT::RUN];                              // element `wave` of the lane's tiles
+#pragma unroll
+  for (int f = 0; f < JT::RUN; ++f) {
+    x[f] = 0.f;
+    for (int v = 0; v < SPREAD; ++v) x[f] += sums[v][f][lane][wave];
+  }
+  j.store(a, x, l == 0.f ? 0.f : 1.f / l, wave, h);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
@@ -1124,16 +1204,16 @@ static void launch(const Shape& s, const AttnArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)a.workers), threads(64 * AT_WAVES), join((unsigned)a.workers, (unsigned)(s.rows / 16 * CHUNKS));
   if (s.kind == 0) {
     hipLaunchKernelGGL((attend_kernel<T, D, 1, true>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 16, 8>), join, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((join_many_kernel<T, D, 16>), join, dim3(512), 0, st, a);
   } else if (s.kind == 1) {
     hipLaunchKernelGGL((attend_kernel<T, D, 2, true>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 32, 4>), join, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((join_many_kernel<T, D, 32>), join, dim3(512), 0, st, a);
   } else if constexpr (std::is_same<T, bf16>::value && D >= 128) {
     hipLaunchKernelGGL((prompt_kernel<D>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, Prompt<D>::R, 1>), join, dim3(64), 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, Prompt<D>::R>), join, dim3(64), 0, st, a);
   } else {
     hipLaunchKernelGGL((attend_kernel<T, D, 2, false>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 128, 1>), join, dim3(64), 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, 128>), join, dim3(64), 0, st, a);
   }
 }
 
