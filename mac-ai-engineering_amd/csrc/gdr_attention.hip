@@ -48,7 +48,7 @@ struct AttnArgs {
   const uint8_t* cache;
   const int *blocks, *lens, *starts;             // starts null: request r's one query is row r
   float* part;                                   // [2 workers][R rows][D + 2]: O, then m and the sum
-  int4* records;                                 // [workers]: {request, head and row group, last worker, 1 if any}
+  int4* records;                                 // [workers][2]: see Walk::end
   int64_t q_row, q_head;                         // strides in elements
   int64_t T, B, W, pages;
   int Hq, Hk, page, page_shift, workers;
@@ -185,7 +185,7 @@ struct Walk {
   Place at;
   int64_t x0, x1, before, r, u0, u1, stop;       // the line: where the stretch stands and ends, the row group, the piece
   bool opening;                                  // the stretch's first piece, which may have begun in another
-  int4 record;
+  int4 record, record2;
   Req x;
   int head, j, ka, kb, kmin;                     // row group; keys ka .. kb - 1, of which every row sees those below kmin
 
@@ -200,7 +200,7 @@ struct Walk {
     before = at.before;
     r = at.r;
     opening = true;
-    record = {0, 0, 0, 0};
+    record = record2 = {0, 0, 0, 0};
   }
 
   __device__ __forceinline__ bool next() {
@@ -235,13 +235,17 @@ struct Walk {
   }
   __device__ __forceinline__ bool whole() const { return x0 == u0 && stop == u1; }
   __device__ __forceinline__ void done() {
-    if (x0 == u0 && stop != u1)                  // a row group that others go on with begins here
-      record = {(int)r, head * x.groups + j, (int)div64(u1 - 1, at.share), opening ? 1 : 2};
+    if (x0 == u0 && stop != u1) {                // a row group that others go on with begins here
+      record = {1, (int)div64(u1 - 1, at.share), opening, head};
+      record2 = {x.q0, x.qlen, j, 0};
+    }
     opening = false;
     x0 = stop;
   }
+  // What the joins need to know: {whether such a row group begins here, the last workgroup that has a part of it, whether
+  // this one's is its first piece, its head}, {its request's first query row and queries, its row group}.
   __device__ __forceinline__ void end() const {
-    if (threadIdx.x == 0) a.records[w] = record;
+    if (threadIdx.x == 0) a.records[2 * w] = record, a.records[2 * w + 1] = record2;
   }
 };
 
@@ -526,9 +530,9 @@ __device__ __forceinline__ int channel(int d, int h, int i) {
   return d / RUN * (16 * RUN) + (4 * h + i) * RUN + d % RUN;
 }
 
-// Parts of a row group's results lie as a wave holds them, [R / 16 blocks of rows][D / 16 tiles][64 lanes] of f4 (rows apart,
-// a store was 64 lines of 16 bytes: 5 of the 24 us of the prompts' join and most of what a split piece took to end), then
-// R maxima and R sums.  A workgroup has two: its first piece's and its last's.
+// Parts of a row group's results lie as a wave holds them, [R / 16 blocks of rows][D / 16 tiles][16 rows][4 lanes] of f4
+// (a row's channels together, a store was 64 pieces of 16 bytes in as many lines), then R maxima and R sums.  A workgroup
+// has two: its first piece's and its last's.
 template <int R, int D>
 __device__ __forceinline__ float* part_of(const AttnArgs& a, int w, bool opening) {
   return a.part + (int64_t)(2 * w + (opening ? 0 : 1)) * R * (D + 4);
@@ -559,7 +563,7 @@ __device__ __forceinline__ void write_rows(const AttnArgs& a, const W& k, int lr
         }
     } else if (i < k.x.qlen) {
       float* p = part_of<R, D>(a, k.w, k.opening);
-      f4* q = reinterpret_cast<f4*>(p) + (lrow / 16) * ND * 64 + lane;
+      f4* q = reinterpret_cast<f4*>(p) + (lrow / 16) * ND * 64 + n * 4 + h;
 #pragma unroll
       for (int d = 0; d < ND; ++d) q[d * 64] = o[b][d];
       if (h == 0) p[R * D + lrow] = m[b], p[R * D + R + lrow] = l[b];
@@ -1050,137 +1054,145 @@ __global__ void __launch_bounds__(64 * AT_WAVES, prompt_waves(D)) prompt_kernel(
 }
 
 // ---- joining the parts of row groups that several workgroups worked on ---------------------------------------------
-// Block (w, y) takes 16 rows and one chunk of channels (RUN output tiles) of the group that workgroup w began.
-template <typename T, int D, int R>
+// Block (w, y) takes 16 rows and TILES output tiles of the group that workgroup w began.
+template <typename T, int D, int R, int TILES>
 struct Join {
-  static constexpr int RUN = D < 128 ? D / 16 : 8, ND = D / 16;
-  typedef T run_t __attribute__((ext_vector_type(RUN)));
-  int parts, chunk, lrow;                        // the group's parts; the lane's row
+  static constexpr int ND = D / 16;
+  typedef T run_t __attribute__((ext_vector_type(TILES)));
+  int parts, first, lrow;                        // the group's parts; the first tile; the lane's row
   int64_t out;                                   // where its results go
   bool some, there;                              // whether any of the 16 rows exist, and the lane's
   int w, opening;
 
-  __device__ __forceinline__ Join(const AttnArgs& a, const int4& rec, int n) {
+  __device__ __forceinline__ Join(const AttnArgs& a, const int4& rec, const int4& rec2, int n) {
     w = blockIdx.x;
-    const int block = blockIdx.y / (ND / RUN), G = a.Hq / a.Hk;
-    chunk = blockIdx.y % (ND / RUN);
+    const int block = blockIdx.y / (ND / TILES), G = a.Hq / a.Hk;
+    first = blockIdx.y % (ND / TILES) * TILES;
     lrow = block * 16 + n;
-    const Req x = request<R>(a, rec.x, G);
-    const int head = rec.y / x.groups, j = rec.y - head * x.groups, row = j * R + lrow, i = row / G;
-    some = (j * R + block * 16) / G < x.qlen;
-    there = i < x.qlen;
-    out = ((int64_t)(x.q0 + i) * a.Hq + head * G + row - i * G) * D;
-    parts = rec.z - w + 1;                       // w's last piece, then the first ones of w + 1 .. rec.z
-    opening = rec.w == 1;
+    const int row = rec2.z * R + lrow, i = row / G;
+    some = (rec2.z * R + block * 16) / G < rec2.y;
+    there = i < rec2.y;
+    out = ((int64_t)(rec2.x + i) * a.Hq + rec.w * G + row - i * G) * D;
+    parts = rec.y - w + 1;                       // w's last piece, then the first ones of w + 1 .. rec.y
+    opening = rec.z;
   }
   __device__ __forceinline__ const float* part(const AttnArgs& a, int v) const {
     return part_of<R, D>(a, w + v, v ? true : opening);
   }
   __device__ __forceinline__ const f4* tiles(const AttnArgs& a, int v, int lane) const {
-    return reinterpret_cast<const f4*>(part(a, v)) + (lrow / 16 * ND + chunk * RUN) * 64 + lane;
+    return reinterpret_cast<const f4*>(part(a, v)) + (lrow / 16 * ND + first) * 64 + (lane & 15) * 4 + (lane >> 4);
   }
-  // element e of the lane's RUN tiles, times inv
-  __device__ __forceinline__ void store(const AttnArgs& a, const float (&x)[RUN], float inv, int e, int h) const {
+  // element e of the lane's tiles, times inv
+  __device__ __forceinline__ void store(const AttnArgs& a, const float (&x)[TILES], float inv, int e, int h) const {
     run_t v;
 #pragma unroll
-    for (int f = 0; f < RUN; ++f) v[f] = (T)(x[f] * inv);
-    *reinterpret_cast<run_t*>((T*)a.o + out + channel<D>(chunk * RUN, h, e)) = v;
+    for (int f = 0; f < TILES; ++f) v[f] = (T)(x[f] * inv);
+    *reinterpret_cast<run_t*>((T*)a.o + out + channel<D>(first, h, e)) = v;
   }
 };
 
 // Few parts (row groups of many rows, a wave a block).
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(64) join_kernel(AttnArgs a) {
-  using JT = Join<T, D, R>;
-  const int4 rec = a.records[blockIdx.x];
-  if (!rec.w) return;
+  constexpr int TILES = D < 128 ? D / 16 : 8;
+  using JT = Join<T, D, R, TILES>;
+  const int4 rec = a.records[2 * blockIdx.x], rec2 = a.records[2 * blockIdx.x + 1];
+  if (!rec.x) return;
   const int lane = threadIdx.x, h = lane >> 4;
-  const JT j(a, rec, lane & 15);
+  const JT j(a, rec, rec2, lane & 15);
   if (!j.there) return;
   float top = AT_LOWEST, l = 0.f;
-  for (int v = 0; v < j.parts; ++v) top = fmaxf(top, j.part(a, v)[R * D + j.lrow]);
-  f4 o[JT::RUN];
+  f4 o[TILES];
 #pragma unroll
-  for (int e = 0; e < JT::RUN; ++e) o[e] = f4{0.f, 0.f, 0.f, 0.f};
+  for (int e = 0; e < TILES; ++e) o[e] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
   for (int v = 0; v < j.parts; ++v) {
     const float* p = j.part(a, v);
     const f4* q = j.tiles(a, v, lane);
-    const float f = __builtin_amdgcn_exp2f(p[R * D + j.lrow] - top);
-    l += p[R * D + R + j.lrow] * f;
+    const float m = p[R * D + j.lrow], up = fmaxf(top, m);
+    const float f = __builtin_amdgcn_exp2f(m - up), g = __builtin_amdgcn_exp2f(top - up);
+    top = up;
+    l = l * g + p[R * D + R + j.lrow] * f;
 #pragma unroll
-    for (int e = 0; e < JT::RUN; ++e) o[e] += q[e * 64] * f;
+    for (int e = 0; e < TILES; ++e) o[e] = o[e] * g + q[e * 64] * f;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    float x[JT::RUN];
+    float x[TILES];
 #pragma unroll
-    for (int f = 0; f < JT::RUN; ++f) x[f] = o[f][e];
+    for (int f = 0; f < TILES; ++f) x[f] = o[f][e];
     j.store(a, x, inv, e, h);
   }
 }
 
-// Many parts: one long context leaves a few rows with a hundred of them, and what counts is how many loads are in flight.
-// All threads take the maxima and sums, a part to 16 of them; then each wave one part in WAVES / PAIRS of two tiles.
+// Many parts: one long context leaves a few rows with a hundred of them.  What counts is how many lines are in flight, on
+// how many CUs: a block takes two tiles, a wave a part in 4, BATCH of them at once, and the waves join through LDS.
 template <typename T, int D, int R>
-__global__ void __launch_bounds__(512) join_many_kernel(AttnArgs a) {
-  using JT = Join<T, D, R>;
-  constexpr int WAVES = 8, PAIRS = JT::RUN / 2, SPREAD = WAVES / PAIRS, SLOTS = 32, CHUNK = 128;
-  __shared__ float weight[CHUNK][16], tops[SLOTS][16], totals[SLOTS][16];
-  __shared__ f4 sums[SPREAD][JT::RUN][64];
-  const int4 rec = a.records[blockIdx.x];
-  if (!rec.w) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 4, n = lane & 15, slot = threadIdx.x >> 4;
-  const JT j(a, rec, n);
+__global__ void __launch_bounds__(256) join_many_kernel(AttnArgs a) {
+  using JT = Join<T, D, R, 2>;
+  constexpr int WAVES = 4, BATCH = 12;
+  __shared__ float tops[WAVES][16], totals[WAVES][16];
+  __shared__ f4 sums[WAVES][2][64];
+  const int4 rec = a.records[2 * blockIdx.x], rec2 = a.records[2 * blockIdx.x + 1];
+  if (!rec.x) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 4, n = lane & 15;
+  const JT j(a, rec, rec2, n);
   if (!j.some) return;
   float top = AT_LOWEST, l = 0.f;
-  if (j.there) {
-#pragma unroll 4
-    for (int v = slot; v < j.parts; v += SLOTS) top = fmaxf(top, j.part(a, v)[R * D + j.lrow]);
-  }
-  tops[slot][n] = top;
-  __syncthreads();
-  for (int v = 0; v < SLOTS; ++v) top = fmaxf(top, tops[v][n]);
-  const int pair = wave % PAIRS, first = wave / PAIRS;
   f4 o[2] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
-  for (int v0 = 0; v0 < j.parts; v0 += CHUNK) {
-    const int m = min(CHUNK, j.parts - v0);
-    __syncthreads();                             // the weights before these have been read
-    for (int v = slot; v < m; v += SLOTS) {
-      float f = 0.f;
-      if (j.there) {
-        const float* p = j.part(a, v0 + v);
-        f = __builtin_amdgcn_exp2f(p[R * D + j.lrow] - top);
-        l += p[R * D + R + j.lrow] * f;
-      }
-      weight[v][n] = f;
-    }
-    __syncthreads();
-    if (j.there) {
-#pragma unroll 8
-      for (int v = first; v < m; v += SPREAD) {
-        const f4* q = j.tiles(a, v0 + v, lane) + pair * 2 * 64;
-        const float f = weight[v][n];
-        o[0] += q[0] * f;
-        o[1] += q[64] * f;
-      }
-    }
-  }
-  totals[slot][n] = l;
-  sums[first][pair * 2][lane] = o[0];
-  sums[first][pair * 2 + 1][lane] = o[1];
-  __syncthreads();
-  if (wave >= 4 || !j.there) return;
-  l = 0.f;
-  for (int v = 0; v < SLOTS; ++v) l += totals[v][n];
-  float x[JT::RUN];                              // element `wave` of the lane's tiles
+  if (j.there) {
+    for (int v0 = wave; v0 < j.parts; v0 += WAVES * BATCH) {
+      float m[BATCH], s[BATCH];
+      f4 x[BATCH][2];
 #pragma unroll
-  for (int f = 0; f < JT::RUN; ++f) {
-    x[f] = 0.f;
-    for (int v = 0; v < SPREAD; ++v) x[f] += sums[v][f][lane][wave];
+      for (int i = 0; i < BATCH; ++i) {
+        const int v = v0 + i * WAVES;
+        m[i] = -__builtin_inff();
+        if (v >= j.parts) continue;
+        const float* p = j.part(a, v);
+        const f4* q = j.tiles(a, v, lane);
+        m[i] = p[R * D + j.lrow];
+        s[i] = p[R * D + R + j.lrow];
+        x[i][0] = q[0];
+        x[i][1] = q[64];
+      }
+      float up = top;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) up = fmaxf(up, m[i]);
+      const float g = __builtin_amdgcn_exp2f(top - up);
+      top = up;
+      l *= g;
+      o[0] *= g;
+      o[1] *= g;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        if (v0 + i * WAVES >= j.parts) continue;
+        const float f = __builtin_amdgcn_exp2f(m[i] - top);
+        l += s[i] * f;
+        o[0] += x[i][0] * f;
+        o[1] += x[i][1] * f;
+      }
+    }
   }
-  j.store(a, x, l == 0.f ? 0.f : 1.f / l, wave, h);
+  if (h == 0) tops[wave][n] = top, totals[wave][n] = l;
+  sums[wave][0][lane] = o[0];
+  sums[wave][1][lane] = o[1];
+  __syncthreads();
+  if (!j.there) return;
+  float y[2] = {0.f, 0.f};                       // element `wave` of the lane's tiles
+  top = AT_LOWEST;
+  l = 0.f;
+#pragma unroll
+  for (int v = 0; v < WAVES; ++v) top = fmaxf(top, tops[v][n]);
+#pragma unroll
+  for (int v = 0; v < WAVES; ++v) {
+    const float f = __builtin_amdgcn_exp2f(tops[v][n] - top);
+    l += totals[v][n] * f;
+    y[0] += sums[v][0][lane][wave] * f;
+    y[1] += sums[v][1][lane][wave] * f;
+  }
+  j.store(a, y, l == 0.f ? 0.f : 1.f / l, wave, h);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
@@ -1201,13 +1213,13 @@ static Shape shape_for(int64_t T, int64_t B, int64_t G, int64_t D, int32_t dtype
 template <typename T, int D>
 static void launch(const Shape& s, const AttnArgs& a, hipStream_t st) {
   constexpr int CHUNKS = D < 128 ? 1 : D / 128;
-  const dim3 grid((unsigned)a.workers), threads(64 * AT_WAVES), join((unsigned)a.workers, (unsigned)(s.rows / 16 * CHUNKS));
+  const dim3 grid((unsigned)a.workers), threads(64 * AT_WAVES), join((unsigned)a.workers, (unsigned)(s.rows / 16 * (s.kind < 2 ? D / 32 : CHUNKS)));
   if (s.kind == 0) {
     hipLaunchKernelGGL((attend_kernel<T, D, 1, true>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_many_kernel<T, D, 16>), join, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((join_many_kernel<T, D, 16>), join, dim3(256), 0, st, a);
   } else if (s.kind == 1) {
     hipLaunchKernelGGL((attend_kernel<T, D, 2, true>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_many_kernel<T, D, 32>), join, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((join_many_kernel<T, D, 32>), join, dim3(256), 0, st, a);
   } else if constexpr (std::is_same<T, bf16>::value && D >= 128) {
     hipLaunchKernelGGL((prompt_kernel<D>), grid, threads, 0, st, a);
     hipLaunchKernelGGL((join_kernel<T, D, Prompt<D>::R>), join, dim3(64), 0, st, a);
@@ -1231,7 +1243,7 @@ extern "C" {
 int64_t macai_gdr_kv4_attention_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int32_t dtype) {
   if (T < 1 || B < 1 || Hk < 1 || Hq < Hk || D < 1) return 0;
   const gdr::Shape s = gdr::shape_for(T, B, Hq / Hk, D, dtype);
-  return s.workers * (int64_t)(sizeof(int4) + 2 * s.rows * (D + 4) * sizeof(float));
+  return s.workers * (int64_t)(2 * sizeof(int4) + 2 * s.rows * (D + 4) * sizeof(float));
 }
 
 int macai_gdr_kv4_attention(const void* q, const uint8_t* cache, const int32_t* blocks, const int32_t* lens,
@@ -1262,7 +1274,7 @@ int macai_gdr_kv4_attention(const void* q, const uint8_t* cache, const int32_t* 
   gdr::AttnArgs a{q, o, cache, blocks, lens, starts, nullptr, nullptr, q_row, q_head, T, B, W, pages, (int)Hq, (int)Hk,
                   (int)page, __builtin_ctzll((unsigned long long)page), s.workers, scale * 1.44269504088896341f};
   a.records = (int4*)workspace;
-  a.part = (float*)((char*)workspace + a.workers * sizeof(int4));
+  a.part = (float*)(a.records + 2 * a.workers);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == MACAI_GDR_F32) gdr::launch_width<float>(D, s, a, st);
   else if (dtype == MACAI_GDR_BF16) gdr::launch_width<gdr::bf16>(D, s, a, st);
