@@ -241,7 +241,7 @@ struct AppendArgs {
   Rope rope;
   int64_t rows, pages;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // strides in elements
-  int Hq, Hk, D, page;
+  int Hq, Hk, D, page, page_shift;
 };
 
 // The largest of 4 neighbouring lanes (two exchanges inside the quad).
@@ -250,8 +250,10 @@ __device__ __forceinline__ unsigned quad_max(unsigned x) {
   return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));
 }
 
-// A thread takes 8 channels of one head of q, k or v for TT rows; 4 neighbours hold a group of 32.  Rotated channels of
-// the half layout load their partners too (from the first-level cache: another thread's own).
+// A thread takes 8 channels of one head of q, k or v for TT rows, all their loads issued before the first use; 4 neighbours
+// hold a group of 32.  Rotated channels of the half layout load their partners too (from the first-level cache: another
+// thread's own).  Four rows once one a thread would be APPEND_MANY workgroups or more, eight to a CU.
+constexpr int64_t APPEND_MANY = 2048;
 template <typename T, int TT>
 __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
   const int per = a.D / 8, heads = a.Hq + 2 * a.Hk;
@@ -268,28 +270,49 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
   const bool rot = which < 2 && a.rope.table && ch < w, pairs = rot && !a.rope.interleaved;
   const int partner = ch < half ? ch + half : ch - half;
   const int64_t row0 = (int64_t)blockIdx.x * TT;
-  float x[TT][8], y[TT][8];
+  float x[TT][8], y[TT][8], cs[TT][8], sn[TT][8];
+  int64_t slot[TT];
 #pragma unroll
   for (int i = 0; i < TT; ++i) {
     const int64_t row = min(row0 + i, a.rows - 1);
     load8(src + row * step + ch, x[i]);
     if (pairs) load8(src + row * step + partner, y[i]);
+    slot[i] = which ? a.slots[row] : 0;
+  }
+  if (rot) {
+    const int at = pairs ? (ch < half ? ch : partner) : ch / 2;
+    const float* t[TT];
+#pragma unroll
+    for (int i = 0; i < TT; ++i) t[i] = rope_row(a.rope, min(row0 + i, a.rows - 1));
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+      const float* p = t[i] ? t[i] : a.rope.table;
+      if (pairs) {
+        load8(p + at, cs[i]);
+        load8(p + half + at, sn[i]);
+      } else {
+        const f4 c = *reinterpret_cast<const f4*>(p + at), d = *reinterpret_cast<const f4*>(p + half + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cs[i][e] = c[e], sn[i][e] = d[e];
+      }
+      if (!t[i])
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cs[i][e] = sn[i][e] = __builtin_nanf("");
+    }
   }
 #pragma unroll
   for (int i = 0; i < TT; ++i) {
     const int64_t row = row0 + i;
     if (row >= a.rows) break;
     if (rot) {
-      const float* t = rope_row(a.rope, row);
-      const int at = pairs ? (ch < half ? ch : partner) : ch / 2;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (!pairs && (e & 1)) continue;
-        const int j = pairs ? at + e : at + e / 2;
-        const float c = t ? t[j] : __builtin_nanf(""), s = t ? t[half + j] : __builtin_nanf("");
-        if (!pairs) turn(x[i][e], x[i][e + 1], c, s);
-        else if (ch < half) turn(x[i][e], y[i][e], c, s);
-        else turn(y[i][e], x[i][e], c, s);
+        if (pairs) {
+          if (ch < half) turn(x[i][e], y[i][e], cs[i][e], sn[i][e]);
+          else turn(y[i][e], x[i][e], cs[i][e], sn[i][e]);
+        } else if (e % 2 == 0) {
+          turn(x[i][e], x[i][e + 1], cs[i][e / 2], sn[i][e / 2]);
+        }
       }
     }
     if (which == 0) {
@@ -303,11 +326,10 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
       top = max(top, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);   // a NaN's bits are above an infinity's
     }
     const unsigned byte = kv_scale_byte(quad_max(top));
-    const int64_t slot = a.slots[row];
-    if (slot < 0 || slot >= a.pages * a.page) continue;
+    if (slot[i] < 0 || slot[i] >= a.pages * a.page) continue;
     const unsigned word = kv_encode8(x[i], kv_scale(byte));
-    const int off = (int)(slot % a.page), t = off % KV_SUB, g = ch / 32;
-    uint8_t* sub = a.cache + ((slot / a.page * 2 + which - 1) * a.Hk + h) * kv_page_bytes(a.page, a.D) +
+    const int off = (int)(slot[i] & (a.page - 1)), t = off % KV_SUB, g = ch / 32;
+    uint8_t* sub = a.cache + (((slot[i] >> a.page_shift) * 2 + which - 1) * a.Hk + h) * kv_page_bytes(a.page, a.D) +
                    off / KV_SUB * kv_sub_bytes(a.D);
     if (which == 1) {
       *reinterpret_cast<unsigned*>(sub + kv_key_code(t, ch)) = word;
@@ -328,7 +350,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
 // Slots' keys and values as T [rows, heads, D] each: 8 channels a thread; a slot outside of the cache reads as zeros.
 template <typename T>
 __global__ void __launch_bounds__(256) read_kernel(const uint8_t* cache, const int64_t* slots, T* k, T* v, int64_t rows,
-                                                   int64_t pages, int Hk, int D, int page) {
+                                                   int64_t pages, int Hk, int D, int page, int page_shift) {
   const int per = D / 8;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int ch = (int)(id % per) * 8;
@@ -339,8 +361,8 @@ __global__ void __launch_bounds__(256) read_kernel(const uint8_t* cache, const i
   const int64_t slot = slots[row];
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (slot >= 0 && slot < pages * page) {
-    const int off = (int)(slot % page), t = off % KV_SUB, g = ch / 32;
-    const uint8_t* sub = cache + ((slot / page * 2 + which) * Hk + h) * kv_page_bytes(page, D) +
+    const int off = (int)(slot & (page - 1)), t = off % KV_SUB, g = ch / 32;
+    const uint8_t* sub = cache + (((slot >> page_shift) * 2 + which) * Hk + h) * kv_page_bytes(page, D) +
                          off / KV_SUB * kv_sub_bytes(D);
     unsigned word;
     unsigned byte;
@@ -473,10 +495,17 @@ int macai_gdr_kv4_append(const void* q, const void* k, const void* v, void* qo, 
   const int64_t strides[] = {q_row, q_head, k_row, k_head, v_row, v_head};
   if (!even_strides(strides, 6, dtype)) return fail(MACAI_GDR_EINVAL, "%s: strides must keep 16-byte alignment", what);
   gdr::AppendArgs a{q, k, v, qo, cache, slots, {table, positions, length, (int)width, wide, interleaved}, rows, pages,
-                    q_row, q_head, k_row, k_head, v_row, v_head, (int)Hq, (int)Hk, (int)D, (int)page};
+                    q_row, q_head, k_row, k_head, v_row, v_head, (int)Hq, (int)Hk, (int)D, (int)page,
+                    __builtin_ctzll((unsigned long long)page)};
   const int64_t vecs = ((Hq + 2 * Hk) * (D / 8) + 255) / 256;
   hipStream_t st = (hipStream_t)stream;
-  DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::append_kernel<PT, 1>), dim3((unsigned)rows, (unsigned)vecs), dim3(256), 0, st, a))
+  if (rows * vecs >= gdr::APPEND_MANY) {
+    const dim3 grid((unsigned)((rows + 3) / 4), (unsigned)vecs);
+    DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::append_kernel<PT, 4>), grid, dim3(256), 0, st, a))
+  } else {
+    const dim3 grid((unsigned)rows, (unsigned)vecs);
+    DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::append_kernel<PT, 1>), grid, dim3(256), 0, st, a))
+  }
   return launched(what);
 }
 
@@ -492,7 +521,8 @@ int macai_gdr_kv4_read(const uint8_t* cache, const int64_t* slots, void* k, void
   if (rows > (INT64_C(1) << 38) / (2 * Hk * (D / 8))) return fail(MACAI_GDR_EINVAL, "%s: too many rows", what);
   const dim3 grid((unsigned)((rows * 2 * Hk * (D / 8) + 255) / 256));
   DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::read_kernel<PT>), grid, dim3(256), 0, (hipStream_t)stream, cache, slots,
-                                       (PT*)k, (PT*)v, rows, pages, (int)Hk, (int)D, (int)page))
+                                       (PT*)k, (PT*)v, rows, pages, (int)Hk, (int)D, (int)page,
+                                       __builtin_ctzll((unsigned long long)page)))
   return launched(what);
 }
 
