@@ -105,75 +105,67 @@ struct Place {
   int64_t share, total, r, before;               // cost before request r
 };
 
-// The stretch's length and the request at offset `w * share` of the line (r = B past its end).  All requests' costs are
-// summed by the whole workgroup, 256 at a time.
+// x plus what the lanes below hold of it (an inclusive sum over the wave), by the exchanges of a row of 16 and the two
+// broadcasts between rows.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t add_below(int64_t x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)x, CTRL, ROWS, 0xF, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)((u64)x >> 32), CTRL, ROWS, 0xF, false);
+  return x + (int64_t)((u64)(unsigned)hi << 32 | (unsigned)lo);
+}
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+  x = add_below<0x111, 0xF>(x);                  // row_shr 1, 2, 4, 8
+  x = add_below<0x112, 0xF>(x);
+  x = add_below<0x114, 0xF>(x);
+  x = add_below<0x118, 0xF>(x);
+  x = add_below<0x142, 0xA>(x);                  // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+  return add_below<0x143, 0xC>(x);
+}
+__device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
+  const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)x, lane);
+  const unsigned hi = __builtin_amdgcn_readlane((int)(unsigned)((u64)x >> 32), lane);
+  return (int64_t)((u64)hi << 32 | lo);
+}
+
+// The stretch's length and the request at offset `w * share` of the line (r = B past its end).  Every wave sums all
+// requests' costs, 64 at a time: up to 64 requests are one load and one sum, and no wave waits for another.
 template <int R>
 __device__ __forceinline__ Place find(const AttnArgs& a, int w, int G, int per, int step) {
-  __shared__ int64_t sums[AT_WAVES];
-  __shared__ int64_t found[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lane = threadIdx.x & 63;
+  const auto costs = [&](int64_t r) {
+    if (r >= a.B) return (int64_t)0;
+    const Req x = request<R>(a, r, G);
+    return x.cost(x.groups, per) * a.Hk;
+  };
   Place p;
   p.total = 0;
-  int64_t mine = 0, incl = 0;                    // of the last 256 requests, kept for the second pass
-  const int64_t rounds = (a.B + 255) / 256;
-  for (int64_t i = 0; i < rounds; ++i) {
-    const int64_t r = i * 256 + tid;
-    mine = 0;
-    if (r < a.B) {
-      const Req x = request<R>(a, r, G);
-      mine = x.cost(x.groups, per) * a.Hk;
-    }
-    incl = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int64_t y = __shfl_up(incl, d);
-      if (lane >= d) incl += y;
-    }
-    __syncthreads();
-    if (lane == 63) sums[wave] = incl;
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < AT_WAVES; ++v) p.total += sums[v];
+  int64_t mine = 0, incl = 0;
+  for (int64_t r0 = 0; r0 < a.B; r0 += 64) {
+    mine = costs(r0 + lane);
+    incl = wave_sum(mine);
+    p.total += of_lane(incl, 63);
   }
-  p.share = div64(p.total + a.workers - 1, a.workers);
+  p.share = uniform(div64(p.total + a.workers - 1, a.workers));
   p.share = max((p.share + step - 1) / step * step, (int64_t)step);
+  p.r = a.B;
+  p.before = 0;
   const int64_t at = p.share * w;
-  if (tid == 0) found[0] = a.B, found[1] = 0;
-  __syncthreads();
-  if (at < p.total) {
-    int64_t before = 0;
-    for (int64_t i = 0; i < rounds; ++i) {
-      const int64_t r = i * 256 + tid;
-      if (rounds > 1) {
-        mine = 0;
-        if (r < a.B) {
-          const Req x = request<R>(a, r, G);
-          mine = x.cost(x.groups, per) * a.Hk;
-        }
-        incl = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const int64_t y = __shfl_up(incl, d);
-          if (lane >= d) incl += y;
-        }
-        __syncthreads();
-        if (lane == 63) sums[wave] = incl;
-        __syncthreads();
-      }
-      int64_t b = before + incl - mine;
-#pragma unroll
-      for (int v = 0; v < AT_WAVES; ++v) {
-        if (v < wave) b += sums[v];
-        before += sums[v];
-      }
-      if (at >= b && at < b + mine) found[0] = r, found[1] = b;   // one thread of all
+  if (at >= p.total) return p;
+  int64_t before = 0;
+  for (int64_t r0 = 0; r0 < a.B; r0 += 64) {
+    if (a.B > 64) {
+      mine = costs(r0 + lane);
+      incl = wave_sum(mine);
     }
-    __syncthreads();
+    const u64 past = __ballot(before + incl > at);   // lanes whose request ends past the offset
+    if (past) {
+      const int first = __ffsll((unsigned long long)past) - 1;
+      p.r = r0 + first;
+      p.before = before + of_lane(incl, first) - of_lane(mine, first);
+      return p;
+    }
+    before += of_lane(incl, 63);
   }
-  p.share = uniform(p.share);
-  p.total = uniform(p.total);
-  p.r = uniform(found[0]);
-  p.before = uniform(found[1]);
   return p;
 }
 

@@ -20,31 +20,39 @@ typedef _Float16 f16;
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 
-// 8 values of T (16 or 32 bytes, 16-byte aligned) as floats, and back with one rounding to nearest even.
+// 8 values of T (16 or 32 bytes, 16-byte aligned): as loaded, as floats, and back with one rounding to nearest even.
+template <typename T>
+struct Vec8 {
+  static constexpr int N = 16 / sizeof(T);
+  typedef T part_t __attribute__((ext_vector_type(16 / sizeof(T))));
+  part_t v[8 / N];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int j = 0; j < 8 / N; ++j) v[j] = reinterpret_cast<const part_t*>(p)[j];
+  }
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)v[i / N][i % N];
+  }
+};
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const f4 a = *reinterpret_cast<const f4*>(p), b = *reinterpret_cast<const f4*>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = a[i], x[i + 4] = b[i];
-  } else {
-    typedef T T8 __attribute__((ext_vector_type(8)));
-    const T8 a = *reinterpret_cast<const T8*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
-  }
+  Vec8<T> v;
+  v.load(p);
+  v.floats(x);
 }
-template <typename T>
+// PAST: written past the caches, a long stream that nothing reads back soon.
+template <typename T, bool PAST = false>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<f4*>(p) = f4{x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<f4*>(p + 4) = f4{x[4], x[5], x[6], x[7]};
-  } else {
-    typedef T T8 __attribute__((ext_vector_type(8)));
-    T8 a;
+  typedef typename Vec8<T>::part_t part_t;
+  constexpr int N = Vec8<T>::N;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (T)x[i];
-    *reinterpret_cast<T8*>(p) = a;
+  for (int j = 0; j < 8 / N; ++j) {
+    part_t a;
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = (T)x[j * N + i];
+    if constexpr (PAST) __builtin_nontemporal_store(a, reinterpret_cast<part_t*>(p) + j);
+    else reinterpret_cast<part_t*>(p)[j] = a;
   }
 }
 
@@ -82,31 +90,27 @@ struct RotArgs {
   float sign;             // 1, or -1: the transpose
 };
 
-// A thread takes 16 channels of ROT_HEADS heads of a row that share their angles: a run of 8 and its partners half the
-// width away (interleaved: 16 channels in a row), or 16 that are not rotated.  rotary over 4 x 4,096 tokens, 18 heads of
-// 256, bf16: see the table of cases.
-constexpr int ROT_HEADS = 4;
+// A thread takes 16 channels of a head that share their angles: a run of 8 and its partners half the width away
+// (interleaved: 16 channels in a row), or 16 that are not rotated; its 2 loads, the position's and then the table's are all
+// it waits for.  4 x 4,096 tokens, 18 heads of 256, bf16, forward and backward: 61 us each, 4.9 TB/s of the 5.2 that a copy
+// reaches (4 heads a thread, a row of the table read once for them, 68; stores past the caches 63).
 template <typename T>
 __global__ void __launch_bounds__(256) rotary_kernel(RotArgs a) {
-  const int units = a.D / 16, heads = a.Hq + a.Hk, groups = (heads + ROT_HEADS - 1) / ROT_HEADS;
+  const int units = a.D / 16, heads = a.Hq + a.Hk;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int u = (int)(id % units);
   const int64_t rest = id / units;
-  const int g = (int)(rest % groups);
-  const int64_t row = rest / groups;
+  const int h = (int)(rest % heads);
+  const int64_t row = rest / heads;
   if (row >= a.rows) return;
   const int w = a.rope.width, half = w / 2;
   const bool rot = u < w / 16;
   const int c0 = rot && !a.rope.interleaved ? u * 8 : u * 16, c1 = rot && !a.rope.interleaved ? half + u * 8 : c0 + 8;
-  float x[ROT_HEADS][2][8];
-#pragma unroll
-  for (int j = 0; j < ROT_HEADS; ++j) {
-    const int h = min(g * ROT_HEADS + j, heads - 1);
-    const T* p = h < a.Hq ? (const T*)a.q + row * a.q_row + h * a.q_head
-                          : (const T*)a.k + row * a.k_row + (h - a.Hq) * a.k_head;
-    load8(p + c0, x[j][0]);
-    load8(p + c1, x[j][1]);
-  }
+  const T* p = h < a.Hq ? (const T*)a.q + row * a.q_row + h * a.q_head
+                        : (const T*)a.k + row * a.k_row + (h - a.Hq) * a.k_head;
+  float x[2][8];
+  load8(p + c0, x[0]);
+  load8(p + c1, x[1]);
   if (rot) {
     const float* t = rope_row(a.rope, a.npos == a.rows ? row : row % a.npos);
     float cs[8], sn[8];
@@ -118,22 +122,15 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotArgs a) {
       for (int i = 0; i < 8; ++i) cs[i] = sn[i] = __builtin_nanf("");
     }
 #pragma unroll
-    for (int j = 0; j < ROT_HEADS; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float s = a.sign * sn[i];
-        if (a.rope.interleaved) turn(x[j][i / 4][2 * i % 8], x[j][i / 4][2 * i % 8 + 1], cs[i], s);
-        else turn(x[j][0][i], x[j][1][i], cs[i], s);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float s = a.sign * sn[i];
+      if (a.rope.interleaved) turn(x[i / 4][2 * i % 8], x[i / 4][2 * i % 8 + 1], cs[i], s);
+      else turn(x[0][i], x[1][i], cs[i], s);
+    }
   }
-#pragma unroll
-  for (int j = 0; j < ROT_HEADS; ++j) {
-    const int h = g * ROT_HEADS + j;
-    if (h >= heads) break;
-    T* p = h < a.Hq ? (T*)a.qo + (row * a.Hq + h) * a.D : (T*)a.ko + (row * a.Hk + h - a.Hq) * a.D;
-    store8(p + c0, x[j][0]);
-    store8(p + c1, x[j][1]);
-  }
+  T* o = h < a.Hq ? (T*)a.qo + (row * a.Hq + h) * a.D : (T*)a.ko + (row * a.Hk + h - a.Hq) * a.D;
+  store8(o + c0, x[0]);
+  store8(o + c1, x[1]);
 }
 
 // ---- plan ---------------------------------------------------------------------------------------------------------
@@ -250,100 +247,85 @@ __device__ __forceinline__ unsigned quad_max(unsigned x) {
   return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));
 }
 
-// A thread takes 8 channels of one head of q, k or v for TT rows, all their loads issued before the first use; 4 neighbours
-// hold a group of 32.  Rotated channels of the half layout load their partners too (from the first-level cache: another
-// thread's own).  Four rows once one a thread would be APPEND_MANY workgroups or more, eight to a CU.
-constexpr int64_t APPEND_MANY = 2048;
-template <typename T, int TT>
+// A thread takes 8 channels of one head of q, k or v of a row, its loads issued before the first use; 4 neighbours hold a
+// group of 32.  Rotated channels of the half layout load their partners too (from the first-level cache: another thread's
+// own).  16,383 tokens, 32 + 2 x 8 heads of 128, bf16: 79 us, 4.7 TB/s (two rows a thread 79, four 88).  A q of APPEND_PAST
+// values or more, past what the L2 caches hold, is written past them (79 against 87 us).
+constexpr int64_t APPEND_PAST = INT64_C(1) << 24;
+template <typename T, bool PAST>
 __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
   const int per = a.D / 8, heads = a.Hq + 2 * a.Hk;
   const int vec = blockIdx.y * 256 + threadIdx.x;
   if (vec >= heads * per) return;
+  const int64_t row = blockIdx.x;
   const int ch = vec % per * 8;
   int h = vec / per;
   const int which = h < a.Hq ? 0 : h < a.Hq + a.Hk ? 1 : 2;
   h -= which == 0 ? 0 : which == 1 ? a.Hq : a.Hq + a.Hk;
-  const T* src = (const T*)(which == 0 ? a.q : which == 1 ? a.k : a.v) +
-                 h * (which == 0 ? a.q_head : which == 1 ? a.k_head : a.v_head);
-  const int64_t step = which == 0 ? a.q_row : which == 1 ? a.k_row : a.v_row;
+  const T* src = which == 0   ? (const T*)a.q + row * a.q_row + h * a.q_head
+                 : which == 1 ? (const T*)a.k + row * a.k_row + h * a.k_head
+                              : (const T*)a.v + row * a.v_row + h * a.v_head;
   const int w = a.rope.width, half = w / 2;
   const bool rot = which < 2 && a.rope.table && ch < w, pairs = rot && !a.rope.interleaved;
   const int partner = ch < half ? ch + half : ch - half;
-  const int64_t row0 = (int64_t)blockIdx.x * TT;
-  float x[TT][8], y[TT][8], cs[TT][8], sn[TT][8];
-  int64_t slot[TT];
-#pragma unroll
-  for (int i = 0; i < TT; ++i) {
-    const int64_t row = min(row0 + i, a.rows - 1);
-    load8(src + row * step + ch, x[i]);
-    if (pairs) load8(src + row * step + partner, y[i]);
-    slot[i] = which ? a.slots[row] : 0;
-  }
+  Vec8<T> own, other;
+  f4 cs[2], sn[2];
+  own.load(src + ch);
+  if (pairs) other.load(src + partner);
+  const int64_t slot = which ? a.slots[row] : 0;
+  const float* t = nullptr;
   if (rot) {
-    const int at = pairs ? (ch < half ? ch : partner) : ch / 2;
-    const float* t[TT];
-#pragma unroll
-    for (int i = 0; i < TT; ++i) t[i] = rope_row(a.rope, min(row0 + i, a.rows - 1));
-#pragma unroll
-    for (int i = 0; i < TT; ++i) {
-      const float* p = t[i] ? t[i] : a.rope.table;
-      if (pairs) {
-        load8(p + at, cs[i]);
-        load8(p + half + at, sn[i]);
-      } else {
-        const f4 c = *reinterpret_cast<const f4*>(p + at), d = *reinterpret_cast<const f4*>(p + half + at);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) cs[i][e] = c[e], sn[i][e] = d[e];
-      }
-      if (!t[i])
-#pragma unroll
-        for (int e = 0; e < 8; ++e) cs[i][e] = sn[i][e] = __builtin_nanf("");
-    }
+    t = rope_row(a.rope, row);
+    const f4* p = reinterpret_cast<const f4*>((t ? t : a.rope.table) + (pairs ? (ch < half ? ch : partner) : ch / 2));
+    cs[0] = p[0];
+    sn[0] = p[half / 4];
+    if (pairs) cs[1] = p[1], sn[1] = p[half / 4 + 1];
   }
-#pragma unroll
-  for (int i = 0; i < TT; ++i) {
-    const int64_t row = row0 + i;
-    if (row >= a.rows) break;
-    if (rot) {
+  float x[8];
+  own.floats(x);
+  if (rot) {
+    if (!t) cs[0] = cs[1] = f4(__builtin_nanf(""));
+    if (pairs) {
+      float y[8];
+      other.floats(y);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (pairs) {
-          if (ch < half) turn(x[i][e], y[i][e], cs[i][e], sn[i][e]);
-          else turn(y[i][e], x[i][e], cs[i][e], sn[i][e]);
-        } else if (e % 2 == 0) {
-          turn(x[i][e], x[i][e + 1], cs[i][e / 2], sn[i][e / 2]);
-        }
+        if (ch < half) turn(x[e], y[e], cs[e / 4][e % 4], sn[e / 4][e % 4]);
+        else turn(y[e], x[e], cs[e / 4][e % 4], sn[e / 4][e % 4]);
       }
-    }
-    if (which == 0) {
-      if (a.qo) store8((T*)a.qo + (row * a.Hq + h) * a.D + ch, x[i]);
-      continue;
-    }
-    unsigned top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[i][e] = (float)(T)x[i][e];                              // as the model's type holds it
-      top = max(top, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);   // a NaN's bits are above an infinity's
-    }
-    const unsigned byte = kv_scale_byte(quad_max(top));
-    if (slot[i] < 0 || slot[i] >= a.pages * a.page) continue;
-    const unsigned word = kv_encode8(x[i], kv_scale(byte));
-    const int off = (int)(slot[i] & (a.page - 1)), t = off % KV_SUB, g = ch / 32;
-    uint8_t* sub = a.cache + (((slot[i] >> a.page_shift) * 2 + which - 1) * a.Hk + h) * kv_page_bytes(a.page, a.D) +
-                   off / KV_SUB * kv_sub_bytes(a.D);
-    if (which == 1) {
-      *reinterpret_cast<unsigned*>(sub + kv_key_code(t, ch)) = word;
-      if ((ch & 31) == 0) sub[kv_key_scale(a.D, t, g)] = (uint8_t)byte;
     } else {
-      uint8_t* p = sub + kv_value_code(a.D, t, ch);
-      if (a.D >= 128) {
-        *reinterpret_cast<unsigned*>(p) = word;
-      } else {
-        *reinterpret_cast<unsigned short*>(p) = (unsigned short)word;
-        *reinterpret_cast<unsigned short*>(p + 8) = (unsigned short)(word >> 16);
-      }
-      if ((ch & 31) == 0) sub[kv_value_scale(a.D, t, g)] = (uint8_t)byte;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) turn(x[e], x[e + 1], cs[0][e / 2], sn[0][e / 2]);
     }
+  }
+  if (which == 0) {
+    if (a.qo) store8<T, PAST>((T*)a.qo + (row * a.Hq + h) * a.D + ch, x);
+    return;
+  }
+  unsigned top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = (float)(T)x[e];                                 // as the model's type holds it
+    top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);   // a NaN's bits are above an infinity's
+  }
+  const unsigned byte = kv_scale_byte(quad_max(top));
+  if (slot < 0 || slot >= a.pages * a.page) return;
+  const unsigned word = kv_encode8(x, kv_scale(byte));
+  const int off = (int)(slot & (a.page - 1)), token = off % KV_SUB, g = ch / 32;
+  uint8_t* sub = a.cache + (((slot >> a.page_shift) * 2 + which - 1) * a.Hk + h) * kv_page_bytes(a.page, a.D) +
+                 off / KV_SUB * kv_sub_bytes(a.D);
+  if (which == 1) {
+    *reinterpret_cast<unsigned*>(sub + kv_key_code(token, ch)) = word;
+    if ((ch & 31) == 0) sub[kv_key_scale(a.D, token, g)] = (uint8_t)byte;
+  } else {
+    uint8_t* p = sub + kv_value_code(a.D, token, ch);
+    if (a.D >= 128) {
+      *reinterpret_cast<unsigned*>(p) = word;
+    } else {
+      *reinterpret_cast<unsigned short*>(p) = (unsigned short)word;
+      *reinterpret_cast<unsigned short*>(p + 8) = (unsigned short)(word >> 16);
+    }
+    if ((ch & 31) == 0) sub[kv_value_scale(a.D, token, g)] = (uint8_t)byte;
   }
 }
 
@@ -450,11 +432,11 @@ int macai_gdr_rotary(const void* q, const void* k, void* qo, void* ko, const flo
     if (!aligned16(p)) return fail(MACAI_GDR_EINVAL, "%s: pointers must be 16-byte aligned", what);
   const int64_t strides[] = {q_row, q_head, k_row, k_head};
   if (!even_strides(strides, 4, dtype)) return fail(MACAI_GDR_EINVAL, "%s: strides must keep 16-byte alignment", what);
-  const int64_t groups = (Hq + Hk + gdr::ROT_HEADS - 1) / gdr::ROT_HEADS;
-  if (rows > (INT64_C(1) << 38) / (groups * (D / 16))) return fail(MACAI_GDR_EINVAL, "%s: too many rows", what);
+  const int64_t per = (Hq + Hk) * (D / 16);
+  if (rows > (INT64_C(1) << 38) / per) return fail(MACAI_GDR_EINVAL, "%s: too many rows", what);
   gdr::RotArgs a{q, k, qo, ko, {table, positions, length, (int)width, wide, interleaved}, rows, npos, q_row, q_head, k_row,
                  k_head, (int)Hq, (int)Hk, (int)D, transpose ? -1.f : 1.f};
-  const dim3 grid((unsigned)((rows * groups * (D / 16) + 255) / 256));
+  const dim3 grid((unsigned)((rows * per + 255) / 256));
   DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::rotary_kernel<PT>), grid, dim3(256), 0, (hipStream_t)stream, a))
   return launched(what);
 }
@@ -499,12 +481,11 @@ int macai_gdr_kv4_append(const void* q, const void* k, const void* v, void* qo, 
                     __builtin_ctzll((unsigned long long)page)};
   const int64_t vecs = ((Hq + 2 * Hk) * (D / 8) + 255) / 256;
   hipStream_t st = (hipStream_t)stream;
-  if (rows * vecs >= gdr::APPEND_MANY) {
-    const dim3 grid((unsigned)((rows + 3) / 4), (unsigned)vecs);
-    DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::append_kernel<PT, 4>), grid, dim3(256), 0, st, a))
+  const dim3 grid((unsigned)rows, (unsigned)vecs);
+  if (rows * Hq * D >= gdr::APPEND_PAST) {
+    DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::append_kernel<PT, true>), grid, dim3(256), 0, st, a))
   } else {
-    const dim3 grid((unsigned)rows, (unsigned)vecs);
-    DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::append_kernel<PT, 1>), grid, dim3(256), 0, st, a))
+    DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::append_kernel<PT, false>), grid, dim3(256), 0, st, a))
   }
   return launched(what);
 }

@@ -21,6 +21,7 @@ from ._rotary import DTYPES, _rows, _table_unfit
 
 WIDTHS = (64, 128, 256)
 PAGES = (16, 32, 64, 128, 256)
+_WORK = {}      # bytes of workspace by shape (a call of the library otherwise)
 
 
 def kv4_cache(pages: int, heads: int, width: int, page: int = 64, device="cuda") -> torch.Tensor:
@@ -31,17 +32,20 @@ def kv4_cache(pages: int, heads: int, width: int, page: int = 64, device="cuda")
     return torch.zeros(pages, 2, heads, page * 17 * width // 32, dtype=torch.uint8, device=device)
 
 
+I32, I64 = torch.int32, torch.int64
+
+
 def _page_of(cache, width: int, what: str) -> int:
     """The tokens a page of this cache holds; raises where it is no cache of heads of `width` channels."""
-    if not isinstance(cache, torch.Tensor) or cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[1] != 2:
+    shape = cache.shape if isinstance(cache, torch.Tensor) and cache.dtype == torch.uint8 else ()
+    if len(shape) != 4 or shape[1] != 2:
         raise ValueError(f"macai {what}: the cache must be a uint8 tensor [pages, 2, heads, bytes] (kv4_cache)")
     if width not in WIDTHS:
         raise ValueError(f"macai {what}: the head width must be one of {WIDTHS} (got {width})")
-    page, rest = divmod(cache.shape[3] * 32, 17 * width)
+    page, rest = divmod(shape[3] * 32, 17 * width)
     if rest or page not in PAGES:
-        raise ValueError(f"macai {what}: {cache.shape[3]} bytes are no page of heads of {width}: a page holds one of {PAGES} "
-                         "tokens")
-    if not cache.is_contiguous() or cache.data_ptr() % 16 or cache.shape[0] < 1 or cache.shape[2] < 1:
+        raise ValueError(f"macai {what}: {shape[3]} bytes are no page of heads of {width}: a page holds one of {PAGES} tokens")
+    if not cache.is_contiguous() or cache.data_ptr() % 16 or shape[0] < 1 or shape[2] < 1:
         raise ValueError(f"macai {what}: the cache must be contiguous, 16-byte aligned and not empty")
     return page
 
@@ -51,20 +55,22 @@ def _need(ok: bool, what: str, why: str):
         raise ValueError(f"macai {what}: {why}")
 
 
-def _same_device(what: str, *tensors):
-    dev = tensors[0].device
-    if any(t.device != dev for t in tensors):
-        raise ValueError(f"macai {what}: the tensors must be on one device")
-    if dev.type != "cuda":
+def _device(what: str, t, *others):
+    """Checks that all tensors are on t's device, a HIP device."""
+    dev = t.device
+    for x in others:
+        if x.device != dev:
+            raise ValueError(f"macai {what}: the tensors must be on one device")
+    if not t.is_cuda:
         raise RuntimeError(f"macai's {what} runs on a HIP device (MI355X); got {dev}")
 
 
 def _vector(t, dtype, n, what: str, name: str):
-    """t, checked to be a contiguous tensor of `dtype` [n] (n None: any length)."""
-    _need(isinstance(t, torch.Tensor) and t.dtype == dtype and t.dim() == 1 and (n is None or t.shape[0] == n)
-          and t.is_contiguous(), what, f"{name} must be a contiguous {dtype} tensor [{'n' if n is None else n}]"
-          f" (got {(t.dtype, tuple(t.shape)) if isinstance(t, torch.Tensor) else type(t)})")
-    return t
+    """Checks that t is a contiguous tensor of `dtype` [n] (n None: any length)."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or len(t.shape) != 1 or not t.is_contiguous() or (
+            n is not None and t.shape[0] != n):
+        raise ValueError(f"macai {what}: {name} must be a contiguous {dtype} tensor [{'n' if n is None else n}] "
+                         f"(got {(t.dtype, tuple(t.shape)) if isinstance(t, torch.Tensor) else type(t)})")
 
 
 def kv4_plan(lens, new, blocks, free, head, tokens: int, page: int = 64):
@@ -77,24 +83,27 @@ def kv4_plan(lens, new, blocks, free, head, tokens: int, page: int = 64):
     head above len(free) says so.  Rows past the requests' tokens have the slot -1 and position 0.  The inputs other than
     blocks are left as they are, so a step that is planned again from them comes out the same."""
     w = "kv4_plan"
-    _need(isinstance(blocks, torch.Tensor) and blocks.dtype == torch.int32 and blocks.dim() == 2 and blocks.is_contiguous()
-          and blocks.numel() > 0, w, "blocks must be a contiguous int32 tensor [B, W] that is not empty")
-    B, W = blocks.shape
-    _vector(lens, torch.int32, B, w, "lens")
-    _vector(new, torch.int32, B, w, "new")
-    _vector(free, torch.int32, None, w, "free")
-    _vector(head, torch.int32, 1, w, "head")
-    _need(tokens >= 0 and page >= 1, w, f"need tokens >= 0 and page >= 1 (got {tokens}, {page})")
-    _same_device(w, blocks, lens, new, free, head)
-    i32 = dict(dtype=torch.int32, device=blocks.device)
+    shape = blocks.shape if isinstance(blocks, torch.Tensor) and blocks.dtype == I32 and blocks.is_contiguous() else ()
+    if len(shape) != 2 or 0 in shape:
+        raise ValueError("macai kv4_plan: blocks must be a contiguous int32 tensor [B, W] that is not empty")
+    B, W = shape
+    _vector(lens, I32, B, w, "lens")
+    _vector(new, I32, B, w, "new")
+    _vector(free, I32, None, w, "free")
+    _vector(head, I32, 1, w, "head")
+    if tokens < 0 or page < 1:
+        raise ValueError(f"macai kv4_plan: need tokens >= 0 and page >= 1 (got {tokens}, {page})")
+    _device(w, blocks, lens, new, free, head)
+    dev = blocks.device
     # one allocation of the int32 outputs
-    out = torch.empty(2 * B + 2 + tokens, **i32)
-    starts, total, nxt, positions = out[:B + 1], out[B + 1:2 * B + 1], out[2 * B + 1:2 * B + 2], out[2 * B + 2:]
-    slots = torch.empty(tokens, dtype=torch.int64, device=blocks.device)
-    with _on(blocks.device):
-        N.call("macai_gdr_kv4_plan", lens.data_ptr(), new.data_ptr(), blocks.data_ptr(), free.data_ptr(), head.data_ptr(),
-               starts.data_ptr(), total.data_ptr(), positions.data_ptr(), slots.data_ptr(), nxt.data_ptr(), B, W,
-               free.shape[0], tokens, page, N.stream_of(blocks))
+    starts, total, nxt, positions = torch.empty(2 * B + 2 + tokens, dtype=I32, device=dev).split_with_sizes(
+        (B + 1, B, 1, tokens))
+    slots = torch.empty(tokens, dtype=I64, device=dev)
+    p = starts.data_ptr()
+    with _on(dev):
+        N.call("macai_gdr_kv4_plan", lens.data_ptr(), new.data_ptr(), blocks.data_ptr(), free.data_ptr(), head.data_ptr(), p,
+               p + 4 * (B + 1), p + 4 * (2 * B + 2), slots.data_ptr(), p + 4 * (2 * B + 1), B, W, free.shape[0], tokens, page,
+               N.stream_of(blocks))
     return positions, slots, starts, total, nxt
 
 
@@ -105,40 +114,46 @@ def kv4_append(q, k, v, cache, slots, rope=None, positions=None, interleaved: bo
     launch.  Slots outside of the cache (-1) are skipped.  A group of 32 channels that holds an infinity or a NaN reads as
     NaN.  There is no backward: q, k and v are taken as constants."""
     w = "kv4_append"
-    for name, t in (("k", k), ("v", v)) if q is None else (("q", q), ("k", k), ("v", v)):
-        _need(isinstance(t, torch.Tensor) and t.dim() == 3, w, f"{name} must be a tensor [T, heads, D]")
-    _need(k.dtype in DTYPES and v.dtype == k.dtype and (q is None or q.dtype == k.dtype), w,
-          "q, k and v must share a dtype among float32, bfloat16, float16")
-    T, Hk, D = k.shape
-    _need(v.shape == k.shape and (q is None or (q.shape[0] == T and q.shape[2] == D)), w,
-          f"q, k, v must be [T, heads, D] of the same tokens and width, k and v alike (got "
-          f"{None if q is None else tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)})")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not (isinstance(t, torch.Tensor) and len(t.shape) == 3) and not (name == "q" and t is None):
+            raise ValueError(f"macai kv4_append: {name} must be a tensor [T, heads, D]")
+    dtype, shape = k.dtype, k.shape
+    if dtype not in DTYPES or v.dtype != dtype or (q is not None and q.dtype != dtype):
+        raise ValueError("macai kv4_append: q, k and v must share a dtype among float32, bfloat16, float16")
+    T, Hk, D = shape
+    if v.shape != shape or (q is not None and (q.shape[0] != T or q.shape[2] != D)):
+        raise ValueError("macai kv4_append: q, k, v must be [T, heads, D] of the same tokens and width, k and v alike (got "
+                         f"{None if q is None else tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)})")
     page = _page_of(cache, D, w)
-    _need(cache.shape[2] == Hk, w, f"the cache has {cache.shape[2]} key heads, k and v {Hk}")
-    _vector(slots, torch.int64, T, w, "slots")
-    tensors = [k, v, cache, slots] + ([] if q is None else [q])
-    if rope is not None:
+    pages, _, heads, _ = cache.shape
+    _need(heads == Hk, w, f"the cache has {heads} key heads, k and v {Hk}")
+    _vector(slots, I64, T, w, "slots")
+    if rope is None:
+        _device(w, k, v, cache, slots, *(() if q is None else (q,)))
+        qo = q
+    else:
         _need(q is not None, w, "with a rotary table q is needed")
         why = _table_unfit(rope, positions, D)
-        _need(why is None, w, str(why))
-        _need(tuple(positions.shape) == (T,) and positions.is_contiguous(), w, f"positions must be contiguous [{T}]")
-        tensors += [rope, positions]
-    _same_device(w, *tensors)
-    qo = q if rope is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if why is None and (positions.shape != (T,) or not positions.is_contiguous()):
+            why = f"positions must be contiguous [{T}] (got {tuple(positions.shape)})"
+        _need(why is None, w, why)
+        _device(w, k, v, cache, slots, q, rope, positions)
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
     if T == 0:
         return qo
     k, k_row, k_head = _rows(k, "k")
     v, v_row, v_head = _rows(v, "v")
     if rope is None:
-        q_args, r_args, Hq, q_row, q_head, length, width, wide = (None, None), (None, None), 0, 0, 0, 1, 16, 0
+        pq = pqo = table = pos = None
+        Hq, q_row, q_head, length, width, wide = 0, 0, 0, 1, 16, False
     else:
         q, q_row, q_head = _rows(q, "q")
-        q_args, r_args, Hq = (q.data_ptr(), qo.data_ptr()), (rope.data_ptr(), positions.data_ptr()), q.shape[1]
-        (length, width), wide = rope.shape, int(positions.dtype == torch.int64)
+        pq, pqo, table, pos = q.data_ptr(), qo.data_ptr(), rope.data_ptr(), positions.data_ptr()
+        Hq, (length, width), wide = q.shape[1], rope.shape, positions.dtype == I64
     with _on(k.device):
-        N.call("macai_gdr_kv4_append", q_args[0], k.data_ptr(), v.data_ptr(), q_args[1], cache.data_ptr(), slots.data_ptr(),
-               *r_args, T, cache.shape[0], page, length, Hq, Hk, D, width, q_row, q_head, k_row, k_head, v_row, v_head, wide,
-               int(interleaved), N.dtype_code(k.dtype, True), N.stream_of(k))
+        N.call("macai_gdr_kv4_append", pq, k.data_ptr(), v.data_ptr(), pqo, cache.data_ptr(), slots.data_ptr(), table, pos, T,
+               pages, page, length, Hq, Hk, D, width, q_row, q_head, k_row, k_head, v_row, v_head, wide, bool(interleaved),
+               N.dtype_code(dtype, True), N.stream_of(k))
     return qo
 
 
@@ -147,16 +162,16 @@ def kv4_read(cache, slots, width: int, dtype=torch.bfloat16):
     reads it (bfloat16 and float32 hold it exactly).  Slots outside of the cache give zeros."""
     w = "kv4_read"
     page = _page_of(cache, width, w)
-    _vector(slots, torch.int64, None, w, "slots")
+    _vector(slots, I64, None, w, "slots")
     _need(dtype in DTYPES, w, f"dtype must be float32, bfloat16 or float16 (got {dtype})")
-    _same_device(w, cache, slots)
-    T, Hk = slots.shape[0], cache.shape[2]
+    _device(w, cache, slots)
+    T, (pages, _, Hk, _) = slots.shape[0], cache.shape
     k = torch.empty(T, Hk, width, dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
     if T:
         with _on(cache.device):
-            N.call("macai_gdr_kv4_read", cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), T, cache.shape[0],
-                   page, Hk, width, N.dtype_code(dtype, True), N.stream_of(cache))
+            N.call("macai_gdr_kv4_read", cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), T, pages, page, Hk,
+                   width, N.dtype_code(dtype, True), N.stream_of(cache))
     return k, v
 
 
@@ -171,30 +186,37 @@ def kv4_attention(q, cache, blocks, lens, starts=None, scale: float = None):
     bfloat16 q: products on bf16 operands (keys and values are exact in them) with 32-bit sums.  float16 and float32 q are
     taken as two bf16 terms (16 bits)."""
     w = "kv4_attention"
-    _need(isinstance(q, torch.Tensor) and q.dim() == 3 and q.dtype in DTYPES, w,
-          "q must be a float32, bfloat16 or float16 tensor [T, heads, D]")
+    if not isinstance(q, torch.Tensor) or len(q.shape) != 3 or q.dtype not in DTYPES:
+        raise ValueError("macai kv4_attention: q must be a float32, bfloat16 or float16 tensor [T, heads, D]")
     T, Hq, D = q.shape
     page = _page_of(cache, D, w)
-    Hk = cache.shape[2]
-    _need(Hq >= Hk and Hq % Hk == 0, w, f"the cache's key heads ({Hk}) must divide the query heads ({Hq})")
-    _need(isinstance(blocks, torch.Tensor) and blocks.dtype == torch.int32 and blocks.dim() == 2 and blocks.is_contiguous(), w,
-          "blocks must be a contiguous int32 tensor [B, W]")
-    B, W = blocks.shape
-    _vector(lens, torch.int32, B, w, "lens")
+    pages, _, Hk, _ = cache.shape
+    if Hq < Hk or Hq % Hk:
+        raise ValueError(f"macai kv4_attention: the cache's key heads ({Hk}) must divide the query heads ({Hq})")
+    shape = blocks.shape if isinstance(blocks, torch.Tensor) and blocks.dtype == I32 and blocks.is_contiguous() else ()
+    if len(shape) != 2:
+        raise ValueError("macai kv4_attention: blocks must be a contiguous int32 tensor [B, W]")
+    B, W = shape
+    _vector(lens, I32, B, w, "lens")
     if starts is None:
         _need(T == B, w, f"without starts every request has one query: {T} rows for {B} requests")
-        _same_device(w, q, cache, blocks, lens)
+        _device(w, q, cache, blocks, lens)
     else:
-        _vector(starts, torch.int32, B + 1, w, "starts")
-        _same_device(w, q, cache, blocks, lens, starts)
+        _vector(starts, I32, B + 1, w, "starts")
+        _device(w, q, cache, blocks, lens, starts)
+    dev = q.device
     if T == 0 or B == 0 or W == 0:
-        return torch.zeros(T, Hq, D, dtype=q.dtype, device=q.device)
-    o = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+        return torch.zeros(T, Hq, D, dtype=q.dtype, device=dev)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     q, q_row, q_head = _rows(q, "q")
     code = N.dtype_code(q.dtype, True)
-    work = torch.empty(N.lib().macai_gdr_kv4_attention_workspace(T, B, Hq, Hk, D, code), dtype=torch.uint8, device=q.device)
-    with _on(q.device):
-        N.call("macai_gdr_kv4_attention", q.data_ptr(), cache.data_ptr(), blocks.data_ptr(), lens.data_ptr(), N.ptr(starts),
-               o.data_ptr(), work.data_ptr(), T, B, W, cache.shape[0], page, Hq, Hk, D, q_row, q_head,
-               D ** -0.5 if scale is None else float(scale), code, N.stream_of(q))
+    key = (T, B, Hq, Hk, D, code)
+    size = _WORK.get(key)
+    if size is None:
+        size = _WORK[key] = N.lib().macai_gdr_kv4_attention_workspace(*key)
+    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        N.call("macai_gdr_kv4_attention", q.data_ptr(), cache.data_ptr(), blocks.data_ptr(), lens.data_ptr(),
+               None if starts is None else starts.data_ptr(), o.data_ptr(), work.data_ptr(), T, B, W, pages, page, Hq, Hk, D,
+               q_row, q_head, D ** -0.5 if scale is None else float(scale), code, N.stream_of(q))
     return o

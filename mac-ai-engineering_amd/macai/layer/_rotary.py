@@ -61,11 +61,14 @@ def _rows(t, what: str):
     """t [..., heads, D] as the kernels take it: (tensor, row stride, head stride) with every leading index one row of a
     fixed stride, the channels contiguous and 16-byte vectors aligned -- t itself where it is so, as a slice of a
     projection's output is, a dense copy where not."""
-    shape, s = t.shape, t.stride()
-    v = 16 // t.element_size()
+    shape = t.shape
     if len(shape) < 3:
         raise ValueError(f"macai: {what} must be [..., tokens, heads, channels] (got {tuple(shape)})")
+    s = t.stride()
+    v = 16 // t.element_size()
     if s[-1] == 1 and s[-2] % v == 0 and s[-3] % v == 0 and t.data_ptr() % 16 == 0:
+        if len(shape) == 3:
+            return t, s[0], s[1]
         step, rows = s[-3], shape[-3]
         for n, st in zip(reversed(shape[:-3]), reversed(s[:-3])):
             if n != 1 and st != step * rows:
@@ -78,15 +81,19 @@ def _rows(t, what: str):
     return t, shape[-2] * shape[-1], shape[-1]
 
 
+INTS = (torch.int32, torch.int64)
+
+
 def _table_unfit(table, positions, width_of: int):
     """Why a table and positions do not fit heads of width_of channels, or None."""
-    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype != torch.float32:
+    if not isinstance(table, torch.Tensor) or table.dtype != torch.float32 or len(table.shape) != 2:
         return "the table must be a float32 tensor [positions, width] (rotary_table)"
-    if table.shape[0] < 1 or table.shape[1] % 16 or not 16 <= table.shape[1] <= width_of:
+    length, width = table.shape
+    if length < 1 or width % 16 or not 16 <= width <= width_of:
         return f"the table's width must be a multiple of 16 up to the head's {width_of} (got {tuple(table.shape)})"
     if not table.is_contiguous() or table.data_ptr() % 16:
         return "the table must be contiguous and 16-byte aligned"
-    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in INTS:
         return "positions must be an int32 or int64 tensor"
     return None
 
@@ -95,37 +102,40 @@ def _unfit(q, k, table, positions):
     """Why rotary cannot take these arguments, or None."""
     if not isinstance(q, torch.Tensor) or not isinstance(k, torch.Tensor):
         return "q and k must be tensors"
-    if q.dtype not in DTYPES or k.dtype != q.dtype:
+    dtype, qs, ks = q.dtype, q.shape, k.shape       # read once: a token's call is its host's
+    if dtype not in DTYPES or k.dtype != dtype:
         return f"q and k must share a dtype among float32, bfloat16, float16 (got {q.dtype}, {k.dtype})"
-    if q.dim() < 3 or k.dim() != q.dim() or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
-        return f"q and k must be [..., T, heads, D] of the same tokens and width (got {tuple(q.shape)}, {tuple(k.shape)})"
-    if q.shape[-1] % 16 or not 16 <= q.shape[-1] <= 1024:
-        return f"the head width must be a multiple of 16 up to 1024 (got {q.shape[-1]})"
-    if not 1 <= q.shape[-2] + k.shape[-2] <= 65536:
-        return f"need 1 to 65536 heads (got {q.shape[-2]} and {k.shape[-2]})"
-    why = _table_unfit(table, positions, q.shape[-1])
+    lead, D = qs[:-2], qs[-1] if len(qs) else 0
+    if len(qs) < 3 or len(ks) != len(qs) or lead != ks[:-2] or D != ks[-1]:
+        return f"q and k must be [..., T, heads, D] of the same tokens and width (got {tuple(qs)}, {tuple(ks)})"
+    if D % 16 or not 16 <= D <= 1024:
+        return f"the head width must be a multiple of 16 up to 1024 (got {D})"
+    if not 1 <= qs[-2] + ks[-2] <= 65536:
+        return f"need 1 to 65536 heads (got {qs[-2]} and {ks[-2]})"
+    why = _table_unfit(table, positions, D)
     if why is not None:
         return why
-    lead = tuple(q.shape[:-2])
-    if tuple(positions.shape) != lead and tuple(positions.shape) != lead[-1:]:
-        return f"positions must be {lead} or {lead[-1:]} (got {tuple(positions.shape)})"
-    if len({t.device for t in (q, k, table, positions)}) != 1:
+    if positions.shape != lead and positions.shape != lead[-1:]:
+        return f"positions must be {tuple(lead)} or {tuple(lead[-1:])} (got {tuple(positions.shape)})"
+    dev = q.device
+    if k.device != dev or table.device != dev or positions.device != dev:
         return "q, k, the table and the positions must be on one device"
     return None
 
 
-def _rotate(q, k, table, positions, interleaved: bool, back: bool):
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    rows = q.numel() // max(q.shape[-2] * q.shape[-1], 1) if q.shape[-2] else k.numel() // (k.shape[-2] * k.shape[-1])
+def _rotate(q, k, table, positions, interleaved, back: bool):
+    dense = torch.contiguous_format
+    qo, ko = torch.empty_like(q, memory_format=dense), torch.empty_like(k, memory_format=dense)
+    qs, ks = q.shape, k.shape
+    rows = math.prod(qs[:-2])
     if rows:
         q, q_row, q_head = _rows(q, "q")
         k, k_row, k_head = _rows(k, "k")
+        (length, width), wide = table.shape, positions.dtype == torch.int64
         with _on(q.device):
             N.call("macai_gdr_rotary", q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), table.data_ptr(),
-                   positions.data_ptr(), rows, positions.numel(), table.shape[0], q.shape[-2], k.shape[-2], q.shape[-1],
-                   table.shape[1], q_row, q_head, k_row, k_head, int(positions.dtype == torch.int64), int(interleaved),
-                   int(back), N.dtype_code(q.dtype, True), N.stream_of(q))
+                   positions.data_ptr(), rows, positions.numel(), length, qs[-2], ks[-2], qs[-1], width, q_row, q_head, k_row,
+                   k_head, wide, bool(interleaved), back, N.dtype_code(q.dtype, True), N.stream_of(q))
     return qo, ko
 
 
@@ -159,6 +169,6 @@ def rotary(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, positions: tor
         raise RuntimeError("macai's rotary positions run on a HIP device (MI355X); got " + str(q.device))
     if not positions.is_contiguous():
         positions = positions.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+    if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
         return Rotary.apply(q, k, table, positions, bool(interleaved))
-    return _rotate(q, k, table, positions, bool(interleaved), False)
+    return _rotate(q, k, table, positions, interleaved, False)
