@@ -9,8 +9,8 @@
 // One pass over the keys with the running maximum and sum of the softmax, in 32 bits, on the matrix cores: S^T = K Q^T and
 // O^T = V^T P^T, both v_mfma_f32_16x16x32_bf16 on operands that stay in registers.  Keys and values are decoded to bf16,
 // which holds them exactly (2 bits of mantissa, a power of two), so a bf16 query loses nothing on the way in; P is rounded
-// to bf16 once (at most 2^-8 of it, as the output is).  float16 and float32 queries, and their P, are the sum of two bf16
-// terms each (at most 2^-16 off), at twice the products: the decoded operands are the same.
+// to bf16 once (at most 2^-8 of it, as the output is).  float16 and float32 queries, and their P, are the sum of two and
+// three bf16 terms (at most 2^-16 and 2^-24 off), at as many times the products: the decoded operands are the same.
 //   - S^T's accumulator (lane 16 h + n: query row n, tokens 4 h + i) is P^T's operand for 32 tokens in the order 4 h + 0..3,
 //     16 + 4 h + 0..3; the values are stored so that the same lane loads those tokens.  No exchange of P, no transposition.
 //   - O^T's columns are query rows, so a row's maximum, sum and rescaling are one lane's scalars.
@@ -320,10 +320,16 @@ __device__ __forceinline__ void load_f8(const T* p, float (&x)[8]) {
   }
 }
 
+// bf16 terms that hold a query of type T and its P: 8 bits each.
+template <typename T>
+constexpr int terms_of() {
+  return std::is_same<T, bf16>::value ? 1 : std::is_same<T, f16>::value ? 2 : 3;
+}
+
 // NQ blocks of 16 query rows of a wave: their operands, O^T, reference maxima and sums.
 template <typename T, int D, int NQ>
 struct Rows {
-  static constexpr int TERMS = sizeof(T) == 2 && std::is_same<T, bf16>::value ? 1 : 2;
+  static constexpr int TERMS = terms_of<T>();
   static constexpr int STEPS = D / 32, ND = D / 16;
   bf16x8 q[NQ][TERMS][STEPS];
   f4 o[NQ][ND];
@@ -347,10 +353,12 @@ struct Rows {
         load_f8(p + ch, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float f = there ? v[e] : 0.f;
-          const bf16 hi = (bf16)f;
-          q[b][0][s][e] = hi;
-          if constexpr (TERMS == 2) q[b][1][s][e] = (bf16)(f - (float)hi);
+          float f = there ? v[e] : 0.f;
+#pragma unroll
+          for (int w = 0; w < TERMS; ++w) {
+            q[b][w][s][e] = (bf16)f;
+            f -= (float)q[b][w][s][e];
+          }
         }
       }
 #pragma unroll
@@ -366,7 +374,7 @@ struct Rows {
   template <bool MASKED>
   __device__ __forceinline__ void step(KvTile<D>& t, int t0, int kend, float scale, int lane) {
     using TT = KvTile<D>;
-    constexpr int PT = MASKED ? 2 : TERMS;
+    constexpr int PT = MASKED && TERMS == 1 ? 2 : TERMS;
     const int h = lane >> 4;
     f4 s[NQ][2];
 #pragma unroll
@@ -406,11 +414,13 @@ struct Rows {
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][u][i], scale, -m[b]));
+          float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][u][i], scale, -m[b]));
           l[b] += e;
-          const bf16 hi = (bf16)e;
-          p[b][0][4 * u + i] = hi;
-          if constexpr (PT == 2) p[b][1][4 * u + i] = (bf16)(e - (float)hi);
+#pragma unroll
+          for (int k = 0; k < PT; ++k) {
+            p[b][k][4 * u + i] = (bf16)e;
+            e -= (float)p[b][k][4 * u + i];
+          }
         }
     }
     values(t, p);
@@ -564,13 +574,20 @@ __device__ __forceinline__ void write_rows(const AttnArgs& a, const W& k, int lr
 }
 
 // Waves a SIMD holds of the kernel that streams keys for 16 rows: what keeps enough loads in flight (a tile a wave) and
-// fits the registers.
-constexpr int waves_for(int D) { return D == 256 ? 2 : D == 128 ? 3 : 4; }
+// fits the registers (a float32 query's three terms take the most).
+constexpr int waves_for(int D, int terms) {
+  const int most = D == 256 ? 2 : D == 128 ? 3 : 4;
+  return terms < 3 ? most : most - 1;
+}
+// Where the waves split the rows (and prompt_kernel does not): blocks of 16 rows to a wave, and waves a SIMD holds then.
+constexpr int blocks_of(int D, int terms) { return terms == 1 || (terms == 2 && D < 256) ? 2 : 1; }
+constexpr int row_waves(int D, int terms) { return D == 64 || (terms == 3 && D == 128) || (terms == 2 && D == 256) ? 2 : 1; }
 
 // KEYS: the workgroup's waves take different keys of the same 16 NQ rows and join their results at the end (few rows);
 // else different rows of the same keys (16 NQ each).
 template <typename T, int D, int NQ, bool KEYS>
-__global__ void __launch_bounds__(64 * AT_WAVES, KEYS && NQ == 1 ? waves_for(D) : 1) attend_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(64 * AT_WAVES, !KEYS ? row_waves(D, terms_of<T>()) : NQ == 1 ? waves_for(D, terms_of<T>()) : 1)
+    attend_kernel(AttnArgs a) {
   using RT = Rows<T, D, NQ>;
   constexpr int R = 16 * NQ * (KEYS ? 1 : AT_WAVES), STEP = KEYS ? 32 * AT_WAVES : 32, ND = RT::ND;
   __shared__ f4 join_o[KEYS ? 2 : 1][KEYS ? NQ * ND : 1][64];
@@ -1189,35 +1206,48 @@ __global__ void __launch_bounds__(256) join_many_kernel(AttnArgs a) {
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
 // Rows to a group, how the waves share the work, and the workgroups, by the rows that a request has on average: up to 16,
-// and up to 32, the waves split the keys (the chip is filled by keys alone); above, the rows.
+// and up to 32, the waves split the keys (the chip is filled by keys alone); above, the rows.  (32 float32 rows of 256 do
+// not fit a wave's registers: two groups of 16.)
 struct Shape {
   int kind, rows, workers;                       // kind 0: 16 rows, keys split; 1: 32 rows, keys split; 2: rows split
 };
-static Shape shape_for(int64_t T, int64_t B, int64_t G, int64_t D, int32_t dtype) {
-  const int64_t rows = (T + B - 1) / B * G;
-  if (rows <= 16) return {0, 16, 256 * waves_for((int)D)};
+template <typename T, int D>
+static Shape shape_of(int64_t T_, int64_t B, int64_t G) {
+  constexpr int TERMS = terms_of<T>();
+  constexpr bool WIDE = TERMS == 3 && D == 256;
+  const int64_t rows = (T_ + B - 1) / B * G;
+  if (rows <= (WIDE ? 32 : 16)) return {0, 16, 256 * waves_for(D, TERMS)};
   if (rows <= 32) return {1, 32, 256};
-  if (dtype == MACAI_GDR_BF16 && D >= 128)
-    return {2, D == 256 ? Prompt<256>::R : Prompt<128>::R, 256 * prompt_waves((int)D)};
-  return {2, 128, 256};
+  if constexpr (TERMS == 1 && D >= 128) return {2, Prompt<D>::R, 256 * prompt_waves(D)};
+  return {2, 16 * AT_WAVES * blocks_of(D, TERMS), 256 * row_waves(D, TERMS)};
+}
+static Shape shape_for(int64_t T, int64_t B, int64_t G, int64_t D, int32_t dtype) {
+  const int t = dtype == MACAI_GDR_F32 ? 0 : dtype == MACAI_GDR_BF16 ? 1 : 2;
+  const Shape all[3][3] = {{shape_of<float, 64>(T, B, G), shape_of<float, 128>(T, B, G), shape_of<float, 256>(T, B, G)},
+                           {shape_of<bf16, 64>(T, B, G), shape_of<bf16, 128>(T, B, G), shape_of<bf16, 256>(T, B, G)},
+                           {shape_of<f16, 64>(T, B, G), shape_of<f16, 128>(T, B, G), shape_of<f16, 256>(T, B, G)}};
+  return all[t][D == 64 ? 0 : D == 128 ? 1 : 2];
 }
 
 template <typename T, int D>
 static void launch(const Shape& s, const AttnArgs& a, hipStream_t st) {
-  constexpr int CHUNKS = D < 128 ? 1 : D / 128;
-  const dim3 grid((unsigned)a.workers), threads(64 * AT_WAVES), join((unsigned)a.workers, (unsigned)(s.rows / 16 * (s.kind < 2 ? D / 32 : CHUNKS)));
+  const unsigned parts = s.rows / 16 * (s.kind < 2 ? D / 32 : D < 128 ? 1 : D / 128);   // of a joined row group, a block each
+  const dim3 grid((unsigned)a.workers), threads(64 * AT_WAVES), join((unsigned)a.workers, parts);
   if (s.kind == 0) {
     hipLaunchKernelGGL((attend_kernel<T, D, 1, true>), grid, threads, 0, st, a);
     hipLaunchKernelGGL((join_many_kernel<T, D, 16>), join, dim3(256), 0, st, a);
   } else if (s.kind == 1) {
-    hipLaunchKernelGGL((attend_kernel<T, D, 2, true>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_many_kernel<T, D, 32>), join, dim3(256), 0, st, a);
+    if constexpr (terms_of<T>() < 3 || D < 256) {
+      hipLaunchKernelGGL((attend_kernel<T, D, 2, true>), grid, threads, 0, st, a);
+      hipLaunchKernelGGL((join_many_kernel<T, D, 32>), join, dim3(256), 0, st, a);
+    }
   } else if constexpr (std::is_same<T, bf16>::value && D >= 128) {
     hipLaunchKernelGGL((prompt_kernel<D>), grid, threads, 0, st, a);
     hipLaunchKernelGGL((join_kernel<T, D, Prompt<D>::R>), join, dim3(64), 0, st, a);
   } else {
-    hipLaunchKernelGGL((attend_kernel<T, D, 2, false>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 128>), join, dim3(64), 0, st, a);
+    constexpr int NQ = blocks_of(D, terms_of<T>());
+    hipLaunchKernelGGL((attend_kernel<T, D, NQ, false>), grid, threads, 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, 16 * AT_WAVES * NQ>), join, dim3(64), 0, st, a);
   }
 }
 

@@ -184,7 +184,7 @@ def kv4_attention(q, cache, blocks, lens, starts=None, scale: float = None):
     them gives that request NaN.  There is no backward: it is the form for serving.
 
     bfloat16 q: products on bf16 operands (keys and values are exact in them) with 32-bit sums.  float16 and float32 q are
-    taken as two bf16 terms (16 bits)."""
+    taken as two and three bf16 terms (16 and 24 bits)."""
     w = "kv4_attention"
     if not isinstance(q, torch.Tensor) or len(q.shape) != 3 or q.dtype not in DTYPES:
         raise ValueError("macai kv4_attention: q must be a float32, bfloat16 or float16 tensor [T, heads, D]")
