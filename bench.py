@@ -1,7 +1,7 @@
 """Benchmark of the MI355X gated delta rule: the drop-in's forward + backward at BASELINE config 1.
 
     python bench.py [--gpus 1] [--steps K] [--warmup W] [--no-cpu] [--config 1|2|3|4] [--hv 16|32] [--grouped]
-                    [--packed uniform|ragged] [--stored] [--producers] [--ceilings]
+                    [--packed uniform|ragged] [--stored] [--producers] [--attention] [--ceilings]
 
 A step = one call of macai.gated_delta.chunk_gated_delta_rule (use_qk_l2norm_in_kernel=True, bf16 q/k/v, fp32 g and
 beta) followed by its backward for a seeded upstream gradient dO (torch.autograd.grad, so no gradient accumulation),
@@ -511,6 +511,79 @@ def bench_producers(cfg, reps=20):
     print(json.dumps(line))
 
 
+def attention_bytes(lens, Hq, Hk, D, layers, es=2):
+    """Algorithmic bytes of a step that generates one token a request: a layer reads its cache once (4 bits a channel and
+    a scale byte for 32, keys and values) and q, k, v, writes the token's codes and o."""
+    B = len(lens)
+    return layers * (sum(lens) * 2 * Hk * D * 17 // 32 + B * 2 * Hk * D * 17 // 32 + B * (2 * Hq + 2 * Hk) * D * es)
+
+
+def bench_attention(args):
+    """The attention layers of a serving step: 64 requests of 1,024 to 8,192 tokens held in 4 bits, one token a request.
+    The prompts fill the caches through the same calls, 2,048 tokens at a time; then a step is kv4_plan and, for each
+    layer, kv4_append (rotary positions, 4-bit storage) and kv4_attention, launched by Python and as a captured graph
+    whose replays go on from each other's lengths."""
+    from macai.layer import kv4_append, kv4_attention, kv4_cache, kv4_plan, rotary_table
+    dev = torch.device("cuda", 0)
+    torch.cuda.set_device(dev)
+    B, Hq, Hk, D, page, layers, chunk = 64, 16, 2, 256, 64, 4, 2048
+    gen = torch.Generator(device=dev).manual_seed(11)
+    lens0 = [1024 + 7168 * r // (B - 1) for r in range(B)]
+    W = -(-(max(lens0) + 2 * (args.steps + args.warmup) + 2) // page)
+    i32 = dict(dtype=torch.int32, device=dev)
+    free = torch.randperm(B * W, device=dev, generator=gen, dtype=torch.int32)
+    blocks, head, lens = torch.zeros(B, W, **i32), torch.zeros(1, **i32), torch.zeros(B, **i32)
+    caches = [kv4_cache(B * W, Hk, D, page, dev) for _ in range(layers)]
+    rope = rotary_table(D // 4, W * page, 1e7, device=dev)
+
+    def step(qkv, new, lens, head):
+        positions, slots, starts, total, head = kv4_plan(lens, new, blocks, free, head, qkv.shape[0], page)
+        for cache in caches:
+            q = kv4_append(qkv[:, :Hq], qkv[:, Hq:Hq + Hk], qkv[:, Hq + Hk:], cache, slots, rope, positions)
+            o = kv4_attention(q, cache, blocks, total, starts)
+        return o, total, head
+
+    for at in range(0, max(lens0), chunk):
+        new = [min(max(n - at, 0), chunk) for n in lens0]
+        qkv = torch.randn(sum(new), Hq + 2 * Hk, D, device=dev, generator=gen, dtype=torch.bfloat16)
+        _, lens, head = step(qkv, torch.tensor(new, **i32), lens, head)
+    del qkv
+    qkv = torch.randn(B, Hq + 2 * Hk, D, device=dev, generator=gen, dtype=torch.bfloat16)
+    one = torch.ones(B, **i32)
+
+    def go_on():
+        _, total, nxt = step(qkv, one, lens, head)
+        lens.copy_(total)
+        head.copy_(nxt)
+
+    for _ in range(args.warmup):
+        go_on()
+    sec_eager = _events_time(go_on, args.steps)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        go_on()
+    for _ in range(args.warmup):
+        graph.replay()
+    before = lens.tolist()
+    sec = _events_time(graph.replay, args.steps)
+    after = lens.tolist()
+    if int(head) > free.numel() or [b - a for a, b in zip(before, after)] != [args.steps + 1] * B:
+        raise RuntimeError("bench.py --attention: the cache ran out of pages, or replays did not go on from each other")
+    nbytes = attention_bytes([(a + b) // 2 for a, b in zip(before, after)], Hq, Hk, D, layers)
+    line = {"metric": f"attention layers' decode step GB/s ({layers} layers, B{B}, 1,024-8,192 tokens in 4 bits, Hq{Hq}, "
+                      f"Hk{Hk}, d{D}, bf16)",
+            "value": round(nbytes / sec / 1e9, 1), "unit": "GB/s", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup,
+            "ms_per_step": round(sec * 1e3, 4), "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
+            "dtype": "bf16", "data": "synthetic",
+            "config": {"workload": "plan, then rotary + 4-bit append + paged attention in each layer, as a graph", "B": B,
+                       "Hq": Hq, "Hk": Hk, "D": D, "page": page, "layers": layers, "tokens_held": sum(after)},
+            "roofline": {"kernel": "the whole step", "timing": "HIP events around graph replays", "bound": "hbm",
+                         "achieved": round(nbytes / sec / 1e9, 1), "peak": HBM_PEAK / 1e9, "unit": "GB/s",
+                         "frac": round(nbytes / sec / HBM_PEAK, 4), "traffic": None},
+            "bytes_per_step": nbytes, "tokens_per_s": round(B / sec, 1), "eager_ms_per_step": round(sec_eager * 1e3, 4)}
+    print(json.dumps(line), flush=True)
+
+
 def bench_ceilings(args, mib=1024, reps=10):
     """The device's own streaming rates (macai_gdr_probe_stream: read-only, write-only and copy over `mib` MiB in
     16-byte units, grid-stride; the best of a few workgroup counts, each timed with HIP events over `reps` launches),
@@ -684,6 +757,9 @@ def main():
                          "lengths with the same total")
     ap.add_argument("--producers", action="store_true",
                     help="time the rule's producers (the convolution path and the gates) instead of the rule")
+    ap.add_argument("--attention", action="store_true",
+                    help="time a serving step's attention layers (block plan, rotary positions, 4-bit paged cache and the "
+                         "attention over it) instead of the rule")
     ap.add_argument("--f32-compute", action="store_true",
                     help="run the bf16 inputs on the float32 kernels (op.BF16_OPERANDS = False, the reference's own "
                          "precision) and report that step's time only")
@@ -704,6 +780,9 @@ def main():
         return
     if args.producers:
         bench_producers(args.config)
+        return
+    if args.attention:
+        bench_attention(args)
         return
     if args.config == 3:
         bench_prefill(args)

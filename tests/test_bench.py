@@ -108,3 +108,10 @@ def test_bench_draws_the_oracle_generators_inputs():
     ref = gdr.config_inputs(1)
     for n in ("query", "key", "value", "g", "beta", "do"):
         assert torch.equal(mine[n], ref[n]), n
+
+
+def test_attention_step_bytes():
+    """A layer over 64 tokens held of 2 key heads of 128: 136 bytes a token and head for keys and values, the new token's
+    as many, and q, k, v and o of one token in bf16."""
+    assert bench.attention_bytes([64], 16, 2, 128, 1) == 64 * 2 * 136 + 2 * 136 + (16 + 16 + 2 + 2) * 128 * 2
+    assert bench.attention_bytes([64, 1], 16, 2, 128, 3) == 3 * (65 * 272 + 2 * (272 + 36 * 256))
