@@ -10,6 +10,8 @@
 // All are streams: every byte crosses once, and none computes enough to show.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "gdr_abi.h"
 #include "gdr_common.h"
 #include "gdr_kv4.h"
@@ -329,17 +331,16 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
   }
 }
 
-// Slots' keys and values as T [rows, heads, D] each: 8 channels a thread; a slot outside of the cache reads as zeros.
+// Slots' keys and values as T [rows, heads, D] each: 8 channels a thread, whole rows a block, so that a thread's place is
+// one 32-bit division; a slot outside of the cache reads as zeros.  Neighbouring rows mostly share lines of the cache: with
+// many rows a block takes 4 at least, and 16 neighbouring blocks are blocks of one die, whose L2 holds a line for all of
+// them (16,383 rows of 8 heads of 128: 20.4 us, 4.1 TB/s; 28.5 a row a block and block after block, 22.5 with the dies alone).
+// With few rows what counts is how many threads there are (64 rows: 2.7 us a row a block, 3.5 four).
+constexpr int64_t READ_MANY = 4096;
 template <typename T>
-__global__ void __launch_bounds__(256) read_kernel(const uint8_t* cache, const int64_t* slots, T* k, T* v, int64_t rows,
-                                                   int64_t pages, int Hk, int D, int page, int page_shift) {
-  const int per = D / 8;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int ch = (int)(id % per) * 8;
-  const int64_t rest = id / per;
-  const int hh = (int)(rest % (2 * Hk)), which = hh >= Hk, h = hh - which * Hk;
-  const int64_t row = rest / (2 * Hk);
-  if (row >= rows) return;
+__device__ __forceinline__ void read_piece(const uint8_t* cache, const int64_t* slots, T* k, T* v, int64_t row, int hh, int ch,
+                                           int64_t pages, int Hk, int D, int page, int page_shift) {
+  const int which = hh >= Hk, h = hh - which * Hk;
   const int64_t slot = slots[row];
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (slot >= 0 && slot < pages * page) {
@@ -368,6 +369,18 @@ __global__ void __launch_bounds__(256) read_kernel(const uint8_t* cache, const i
     }
   }
   store8((which ? v : k) + (row * Hk + h) * D + ch, x);
+}
+template <typename T>
+__global__ void __launch_bounds__(256) read_kernel(const uint8_t* cache, const int64_t* slots, T* k, T* v, int64_t rows,
+                                                   int64_t pages, int Hk, int D, int page, int page_shift, int block_rows) {
+  const int shift = __builtin_ctz(D / 8), pieces = 2 * Hk << shift;
+  const int64_t i16 = blockIdx.x >> 3;           // blocks go to the 8 dies in turn
+  const int64_t block = blockIdx.x >= gridDim.x / 128 * 128 ? blockIdx.x : (i16 / 16 * 8 + (blockIdx.x & 7)) * 16 + i16 % 16;
+  for (int i = threadIdx.x; i < block_rows * pieces; i += 256) {
+    const int r = (unsigned)i / (unsigned)pieces, c = i - r * pieces;
+    const int64_t row = block * block_rows + r;
+    if (row < rows) read_piece(cache, slots, k, v, row, c >> shift, (c & (D / 8 - 1)) * 8, pages, Hk, D, page, page_shift);
+  }
 }
 
 }  // namespace gdr
@@ -500,10 +513,11 @@ int macai_gdr_kv4_read(const uint8_t* cache, const int64_t* slots, void* k, void
   if (!aligned16(cache) || !aligned16(k) || !aligned16(v))
     return fail(MACAI_GDR_EINVAL, "%s: pointers must be 16-byte aligned", what);
   if (rows > (INT64_C(1) << 38) / (2 * Hk * (D / 8))) return fail(MACAI_GDR_EINVAL, "%s: too many rows", what);
-  const dim3 grid((unsigned)((rows * 2 * Hk * (D / 8) + 255) / 256));
+  const int64_t block_rows = std::max<int64_t>(256 / (2 * Hk * (D / 8)), rows < gdr::READ_MANY ? 1 : 4);
+  const dim3 grid((unsigned)((rows + block_rows - 1) / block_rows));
   DISPATCH_T(dtype, hipLaunchKernelGGL((gdr::read_kernel<PT>), grid, dim3(256), 0, (hipStream_t)stream, cache, slots,
                                        (PT*)k, (PT*)v, rows, pages, (int)Hk, (int)D, (int)page,
-                                       __builtin_ctzll((unsigned long long)page)))
+                                       __builtin_ctzll((unsigned long long)page), (int)block_rows))
   return launched(what);
 }
 
