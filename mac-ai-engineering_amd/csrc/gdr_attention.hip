@@ -71,7 +71,7 @@ struct Req {
 template <int R>
 __device__ __forceinline__ Req request(const AttnArgs& a, int64_t r, int G) {
   Req x;
-  x.begin = R <= 32 ? 128 : 256;
+  x.begin = R == 16 ? 128 : 256;
   const int64_t most = a.W * a.page;
   x.len = (int)min((int64_t)max(a.lens[r], 0), most);
   if (a.starts) {
@@ -103,23 +103,28 @@ __device__ __forceinline__ int64_t div64(int64_t x, int64_t y) {
 // ---- where a workgroup's stretch begins -----------------------------------------------------------------------------
 struct Place {
   int64_t share, total, r, before;               // cost before request r
+  Req x;                                         // request r
+  bool apart;                                    // a workgroup has one piece:
+  int units, pos;                                // stretches to each of the request's row groups; which of them is its own
 };
 
 // x plus what the lanes below hold of it (an inclusive sum over the wave), by the exchanges of a row of 16 and the two
 // broadcasts between rows.
 template <int CTRL, int ROWS>
-__device__ __forceinline__ int64_t add_below(int64_t x) {
-  const int lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)x, CTRL, ROWS, 0xF, false);
-  const int hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)((u64)x >> 32), CTRL, ROWS, 0xF, false);
-  return x + (int64_t)((u64)(unsigned)hi << 32 | (unsigned)lo);
+__device__ __forceinline__ int below(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t below(int64_t x) {
+  const int lo = below<CTRL, ROWS>((int)(unsigned)x), hi = below<CTRL, ROWS>((int)(unsigned)((u64)x >> 32));
+  return (int64_t)((u64)(unsigned)hi << 32 | (unsigned)lo);
 }
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
-  x = add_below<0x111, 0xF>(x);                  // row_shr 1, 2, 4, 8
-  x = add_below<0x112, 0xF>(x);
-  x = add_below<0x114, 0xF>(x);
-  x = add_below<0x118, 0xF>(x);
-  x = add_below<0x142, 0xA>(x);                  // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
-  return add_below<0x143, 0xC>(x);
+template <typename I>
+__device__ __forceinline__ I wave_sum(I x) {
+  x += below<0x111, 0xF>(x);                     // row_shr 1, 2, 4, 8
+  x += below<0x112, 0xF>(x);
+  x += below<0x114, 0xF>(x);
+  x += below<0x118, 0xF>(x);
+  x += below<0x142, 0xA>(x);                     // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+  return x + below<0x143, 0xC>(x);
 }
 __device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
   const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)x, lane);
@@ -127,34 +132,74 @@ __device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
   return (int64_t)((u64)hi << 32 | lo);
 }
 
+__device__ __forceinline__ Req of_lane(Req x, int lane) {
+  x.q0 = __builtin_amdgcn_readlane(x.q0, lane);
+  x.qlen = __builtin_amdgcn_readlane(x.qlen, lane);
+  x.len = __builtin_amdgcn_readlane(x.len, lane);
+  x.base = __builtin_amdgcn_readlane(x.base, lane);
+  x.groups = __builtin_amdgcn_readlane(x.groups, lane);
+  return x;
+}
+
 // The stretch's length and the request at offset `w * share` of the line (r = B past its end).  Every wave sums all
 // requests' costs, 64 at a time: up to 64 requests are one load and one sum, and no wave waits for another.
+// Where keys are split and there are 4 workgroups or more to a row group, every row group is cut into stretches of its
+// own: a workgroup then has one piece, the longest way through the kernel is not two, and nothing passes 32 bits (one
+// request of 517 tokens, 2 heads of 256: 7.8 us, 12.5 on one line; 16 requests of up to 8,192: 14.8, 20.4).  At 4 the ends of
+// the stretches cost about what second pieces do where contexts are long (64 requests of up to 32,768: 77.1 us, 76.3).
 template <int R>
 __device__ __forceinline__ Place find(const AttnArgs& a, int w, int G, int per, int step) {
   const int lane = threadIdx.x & 63;
-  const auto costs = [&](int64_t r) {
-    if (r >= a.B) return (int64_t)0;
-    const Req x = request<R>(a, r, G);
-    return x.cost(x.groups, per) * a.Hk;
+  const auto load = [&](int64_t r) {
+    Req x = request<R>(a, min(r, a.B - 1), G);
+    if (r >= a.B) x.groups = 0;
+    return x;
   };
   Place p;
-  p.total = 0;
+  p.r = a.B;
+  p.apart = false;
+  Req x;
+  if (R == 16 && a.B <= 64) {
+    x = load(lane);
+    const int64_t groups = of_lane(wave_sum((int64_t)x.groups), 63) * a.Hk;
+    p.apart = groups * 4 <= a.workers;
+    if (p.apart) {
+      // sum of ceil(len / share) <= sum of len / share + groups <= workers; the share is rounded up by more than the
+      // quotient's error, 3 in 2^24
+      const int64_t tokens = of_lane(wave_sum((int64_t)x.groups * x.len), 63) * a.Hk;
+      const float share = (float)tokens * __builtin_amdgcn_rcpf((float)(a.workers - groups)) * (1.f + 0x1p-20f);
+      p.share = ((int)share + step) / step * step;
+      const int units = x.groups ? max((unsigned)(x.len + p.share - 1) / (unsigned)p.share, 1u) : 0;
+      const int mine = units * x.groups * a.Hk, incl = wave_sum(mine);
+      const u64 past = __ballot(incl > w);
+      if (past) {
+        const int first = __ffsll((unsigned long long)past) - 1;
+        p.r = first;
+        p.pos = w - __builtin_amdgcn_readlane(incl - mine, first);
+        p.units = __builtin_amdgcn_readlane(units, first);
+        p.x = of_lane(x, first);
+      }
+      return p;
+    }
+  }
   int64_t mine = 0, incl = 0;
+  p.total = 0;
   for (int64_t r0 = 0; r0 < a.B; r0 += 64) {
-    mine = costs(r0 + lane);
+    x = load(r0 + lane);
+    mine = x.cost(x.groups, per) * a.Hk;
     incl = wave_sum(mine);
     p.total += of_lane(incl, 63);
   }
   p.share = uniform(div64(p.total + a.workers - 1, a.workers));
   p.share = max((p.share + step - 1) / step * step, (int64_t)step);
-  p.r = a.B;
   p.before = 0;
   const int64_t at = p.share * w;
   if (at >= p.total) return p;
   int64_t before = 0;
   for (int64_t r0 = 0; r0 < a.B; r0 += 64) {
     if (a.B > 64) {
-      mine = costs(r0 + lane);
+      x = load(r0 + lane);
+      mine = x.cost(x.groups, per) * a.Hk;
       incl = wave_sum(mine);
     }
     const u64 past = __ballot(before + incl > at);   // lanes whose request ends past the offset
@@ -162,6 +207,7 @@ __device__ __forceinline__ Place find(const AttnArgs& a, int w, int G, int per, 
       const int first = __ffsll((unsigned long long)past) - 1;
       p.r = r0 + first;
       p.before = before + of_lane(incl, first) - of_lane(mine, first);
+      p.x = of_lane(x, first);
       return p;
     }
     before += of_lane(incl, 63);
@@ -175,8 +221,9 @@ struct Walk {
   const AttnArgs& a;
   int w, G, per;
   Place at;
-  int64_t x0, x1, before, r, u0, u1, stop;       // the line: where the stretch stands and ends, the row group, the piece
-  bool opening;                                  // the stretch's first piece, which may have begun in another
+  int64_t x0, x1, before, r, stop;               // the line: where the stretch stands and ends, where the piece does
+  bool opening, begins, ends;                    // the stretch's first piece; the row group begins, ends in this one
+  int goes_to;                                   // the last workgroup that has a part of the row group that begins here
   int4 record, record2;
   Req x;
   int head, j, ka, kb, kmin;                     // row group; keys ka .. kb - 1, of which every row sees those below kmin
@@ -187,17 +234,41 @@ struct Walk {
     G = a.Hq / a.Hk;
     per = (R + G - 1) / G;
     at = find<R>(a, w, G, per, STEP);
-    x0 = at.share * w;
-    x1 = min(x0 + at.share, at.total);
-    before = at.before;
+    if (!at.apart) {
+      x0 = at.share * w;
+      x1 = min(x0 + at.share, at.total);
+      before = at.before;
+    }
     r = at.r;
     opening = true;
     record = record2 = {0, 0, 0, 0};
   }
 
+  // the keys: at most the last row's, both ends of a split rounded to whole steps
+  __device__ __forceinline__ void keys(int64_t from, int64_t to, bool last) {
+    const int rows = min(R, x.qlen * G - j * R), all = x.len - x.qlen + (j * R + rows - 1) / G + 1;
+    kmin = x.len - x.qlen + (j * R) / G + 1;
+    ka = (int)max(from, (int64_t)0) / STEP * STEP;
+    kb = min(all, last ? all : (int)max(to, (int64_t)0) / STEP * STEP);
+  }
   __device__ __forceinline__ bool next() {
+    if (at.apart) {
+      if (!opening || r == a.B) return false;
+      x = at.x;
+      const unsigned each = at.units * x.groups;
+      head = at.pos / each;
+      const int y = at.pos - head * each;
+      j = (unsigned)y / (unsigned)at.units;
+      const int part = y - j * at.units;
+      begins = part == 0;
+      ends = part == at.units - 1;
+      goes_to = w + at.units - 1;
+      keys(part * at.share, (part + 1) * at.share, ends);
+      return true;
+    }
     while (r < a.B && x0 < x1) {
-      x = request<R>(a, r, G);
+      if (r == at.r) x = at.x;
+      else x = request<R>(a, r, G);
       const int64_t each = x.cost(x.groups, per);   // of a head
       if (x0 >= before + each * a.Hk) {
         before += each * a.Hk;
@@ -213,22 +284,20 @@ struct Walk {
         else hi = mid - 1;
       }
       j = lo;
-      u0 = before + head * each + x.cost(j, per);
-      u1 = before + head * each + x.cost(j + 1, per);
+      const int64_t u0 = before + head * each + x.cost(j, per), u1 = before + head * each + x.cost(j + 1, per);
       stop = min(u1, x1);
-      // the keys: at most the last row's, both ends of a split rounded to whole steps
-      const int rows = min(R, x.qlen * G - j * R), all = x.len - x.qlen + (j * R + rows - 1) / G + 1;
-      kmin = x.len - x.qlen + (j * R) / G + 1;
-      ka = max((int)(x0 - u0) - x.begin, 0) / STEP * STEP;
-      kb = min(all, stop == u1 ? all : max((int)(stop - u0) - x.begin, 0) / STEP * STEP);
+      begins = x0 == u0;
+      ends = stop == u1;
+      if (begins && !ends) goes_to = (int)div64(u1 - 1, at.share);
+      keys(x0 - u0 - x.begin, stop - u0 - x.begin, ends);
       return true;
     }
     return false;
   }
-  __device__ __forceinline__ bool whole() const { return x0 == u0 && stop == u1; }
+  __device__ __forceinline__ bool whole() const { return begins && ends; }
   __device__ __forceinline__ void done() {
-    if (x0 == u0 && stop != u1) {                // a row group that others go on with begins here
-      record = {1, (int)div64(u1 - 1, at.share), opening, head};
+    if (begins && !ends) {                       // a row group that others go on with begins here
+      record = {1, goes_to, opening, head};
       record2 = {x.q0, x.qlen, j, 0};
     }
     opening = false;
@@ -540,11 +609,11 @@ __device__ __forceinline__ float* part_of(const AttnArgs& a, int w, bool opening
   return a.part + (int64_t)(2 * w + (opening ? 0 : 1)) * R * (D + 4);
 }
 
-// A wave's 16 NQ rows from lrow0 of the row group on: whole results to o, parts to the workspace.
-template <typename T, int D, int NQ, int R, typename W>
-__device__ __forceinline__ void write_rows(const AttnArgs& a, const W& k, int lrow0, const f4 (&o)[NQ][D / 16],
+// 16 NQ rows from lrow0 of the row group on, ND output tiles from tile0 on: whole results to o, parts to the workspace.
+template <typename T, int D, int NQ, int R, int ND, typename W>
+__device__ __forceinline__ void write_rows(const AttnArgs& a, const W& k, int lrow0, int tile0, const f4 (&o)[NQ][ND],
                                            const float (&m)[NQ], const float (&l)[NQ], int lane) {
-  constexpr int RUN = D < 128 ? D / 16 : 8, ND = D / 16;
+  constexpr int LONG = D < 128 ? D / 16 : 8, RUN = ND < LONG ? ND : LONG;   // a lane's channels in a row, of these tiles
   typedef T run_t __attribute__((ext_vector_type(RUN)));
   const int h = lane >> 4, n = lane & 15;
 #pragma unroll
@@ -561,36 +630,37 @@ __device__ __forceinline__ void write_rows(const AttnArgs& a, const W& k, int lr
           run_t v;
 #pragma unroll
           for (int f = 0; f < RUN; ++f) v[f] = (T)(o[b][c * RUN + f][e] * inv);
-          *reinterpret_cast<run_t*>(p + channel<D>(c * RUN, h, e)) = v;
+          *reinterpret_cast<run_t*>(p + channel<D>(tile0 + c * RUN, h, e)) = v;
         }
     } else if (i < k.x.qlen) {
       float* p = part_of<R, D>(a, k.w, k.opening);
-      f4* q = reinterpret_cast<f4*>(p) + (lrow / 16) * ND * 64 + n * 4 + h;
+      f4* q = reinterpret_cast<f4*>(p) + (lrow / 16 * (D / 16) + tile0) * 64 + n * 4 + h;
 #pragma unroll
       for (int d = 0; d < ND; ++d) q[d * 64] = o[b][d];
-      if (h == 0) p[R * D + lrow] = m[b], p[R * D + R + lrow] = l[b];
+      if (h == 0 && tile0 == 0) p[R * D + lrow] = m[b], p[R * D + R + lrow] = l[b];
     }
   }
 }
 
 // Waves a SIMD holds of the kernel that streams keys for 16 rows: what keeps enough loads in flight (a tile a wave) and
 // fits the registers (a float32 query's three terms take the most).
-constexpr int waves_for(int D, int terms) {
+constexpr int key_waves(int D, int terms) {
   const int most = D == 256 ? 2 : D == 128 ? 3 : 4;
   return terms < 3 ? most : most - 1;
 }
 // Where the waves split the rows (and prompt_kernel does not): blocks of 16 rows to a wave, and waves a SIMD holds then.
-constexpr int blocks_of(int D, int terms) { return terms == 1 || (terms == 2 && D < 256) ? 2 : 1; }
+constexpr int row_blocks(int D, int terms) { return terms == 1 || (terms == 2 && D < 256) ? 2 : 1; }
 constexpr int row_waves(int D, int terms) { return D == 64 || (terms == 3 && D == 128) || (terms == 2 && D == 256) ? 2 : 1; }
 
-// KEYS: the workgroup's waves take different keys of the same 16 NQ rows and join their results at the end (few rows);
+// KEYS: the workgroup's waves take different keys of the same 16 rows and join their results at the end (few rows);
 // else different rows of the same keys (16 NQ each).
-template <typename T, int D, int NQ, bool KEYS>
-__global__ void __launch_bounds__(64 * AT_WAVES, !KEYS ? row_waves(D, terms_of<T>()) : NQ == 1 ? waves_for(D, terms_of<T>()) : 1)
+template <typename T, int D, bool KEYS>
+__global__ void __launch_bounds__(64 * AT_WAVES, KEYS ? key_waves(D, terms_of<T>()) : row_waves(D, terms_of<T>()))
     attend_kernel(AttnArgs a) {
+  constexpr int NQ = KEYS ? 1 : row_blocks(D, terms_of<T>());
   using RT = Rows<T, D, NQ>;
   constexpr int R = 16 * NQ * (KEYS ? 1 : AT_WAVES), STEP = KEYS ? 32 * AT_WAVES : 32, ND = RT::ND;
-  __shared__ f4 join_o[KEYS ? 2 : 1][KEYS ? NQ * ND : 1][64];
+  __shared__ f4 join_o[KEYS ? AT_WAVES : 1][KEYS ? NQ * ND : 1][64];
   __shared__ float join_m[KEYS ? AT_WAVES : 1][NQ][16], join_l[KEYS ? AT_WAVES : 1][NQ][16];
   const int lane = threadIdx.x & 63, h = lane >> 4, n = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -633,49 +703,41 @@ __global__ void __launch_bounds__(64 * AT_WAVES, !KEYS ? row_waves(D, terms_of<T
       fetch(t0, tile);
     }
     rw.end();
-    if constexpr (KEYS) {                        // join the waves: 2, 3 into 0, 1, then 1 into 0
+    if constexpr (KEYS) {                        // join the waves: each takes a quarter of the output tiles
+      constexpr int NT = ND / AT_WAVES;
       __syncthreads();                           // the piece before has been read
 #pragma unroll
-      for (int b = 0; b < NQ; ++b)
+      for (int b = 0; b < NQ; ++b) {
         if (h == 0) join_m[wave][b][n] = bad ? __builtin_nanf("") : rw.m[b], join_l[wave][b][n] = rw.l[b];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) join_o[wave][b * ND + d][lane] = rw.o[b][d];
+      }
       __syncthreads();
+      f4 o[NQ][NT];
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
-        float m = AT_LOWEST, l = 0.f;
-        bool poison = false;
-        for (int v = 0; v < AT_WAVES; ++v) {
-          poison |= __isnanf(join_m[v][b][n]);
-          m = fmaxf(m, join_m[v][b][n]);
-        }
-        for (int v = 0; v < AT_WAVES; ++v) l += join_l[v][b][n] * __builtin_amdgcn_exp2f(join_m[v][b][n] - m);
-        const float f = __builtin_amdgcn_exp2f(rw.m[b] - m);
-        rw.m[b] = m;
-        rw.l[b] = poison ? __builtin_nanf("") : l;
+        rw.m[b] = AT_LOWEST;
+        rw.l[b] = 0.f;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) rw.o[b][d] *= f;
+        for (int v = 0; v < AT_WAVES; ++v) rw.m[b] = fmaxf(rw.m[b], join_m[v][b][n]);
+#pragma unroll
+        for (int d = 0; d < NT; ++d) o[b][d] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < AT_WAVES; ++v) {     // a wave that read a bad page number has a NaN here, which stays
+          const float f = __builtin_amdgcn_exp2f(join_m[v][b][n] - rw.m[b]);
+          rw.l[b] += join_l[v][b][n] * f;
+#pragma unroll
+          for (int d = 0; d < NT; ++d) o[b][d] += join_o[v][b * ND + wave * NT + d][lane] * f;
+        }
       }
+      write_rows<T, D, NQ, R, NT>(a, k, 0, wave * NT, o, rw.m, rw.l, lane);
+    } else {
+      if (bad) {
 #pragma unroll
-      for (int half = 2; half >= 1; half /= 2) {
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-          for (int b = 0; b < NQ; ++b)
-#pragma unroll
-            for (int d = 0; d < ND; ++d) join_o[wave - half][b * ND + d][lane] = rw.o[b][d];
-        }
-        __syncthreads();
-        if (wave < half) {
-#pragma unroll
-          for (int b = 0; b < NQ; ++b)
-#pragma unroll
-            for (int d = 0; d < ND; ++d) rw.o[b][d] += join_o[wave][b * ND + d][lane];
-        }
-        __syncthreads();
+        for (int b = 0; b < NQ; ++b) rw.l[b] = __builtin_nanf("");
       }
-    } else if (bad) {
-#pragma unroll
-      for (int b = 0; b < NQ; ++b) rw.l[b] = __builtin_nanf("");
+      write_rows<T, D, NQ, R, ND>(a, k, wave * 16 * NQ, 0, rw.o, rw.m, rw.l, lane);
     }
-    if (!KEYS || wave == 0) write_rows<T, D, NQ, R>(a, k, KEYS ? 0 : wave * 16 * NQ, rw.o, rw.m, rw.l, lane);
     k.done();
   }
   k.end();
@@ -918,8 +980,8 @@ struct Prompt {
         }
   }
 
-  // O^T += V^T P^T from a buffer of operands, four fragments in flight (with two, each pair of reads waited out its latency:
-  // FRAG_US).
+  // O^T += V^T P^T from a buffer of operands, four fragments in flight (two took 128 us where four take 125, at heads of 128; heads of
+  // 256 have registers for two).
   __device__ __forceinline__ void values(const unsigned (*buf)[64][4], const bf16x8 (&p)[NQ][KB], int lane) {
     constexpr int N = KB * ND, AHEAD = D == 256 ? 2 : 4;
     u32x4_t v[AHEAD];
@@ -1055,7 +1117,7 @@ __global__ void __launch_bounds__(64 * AT_WAVES, prompt_waves(D)) prompt_kernel(
       w.l[b] += __shfl_xor(w.l[b], 32);
       if (lost) w.l[b] = __builtin_nanf("");
     }
-    write_rows<bf16, D, NQ, R>(a, k, wave * 16 * NQ, w.o, w.m, w.l, lane);
+    write_rows<bf16, D, NQ, R, D / 16>(a, k, wave * 16 * NQ, 0, w.o, w.m, w.l, lane);
     __syncthreads();                             // everything of this piece has been read
     k.done();
   }
@@ -1205,21 +1267,22 @@ __global__ void __launch_bounds__(256) join_many_kernel(AttnArgs a) {
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
-// Rows to a group, how the waves share the work, and the workgroups, by the rows that a request has on average: up to 16,
-// and up to 32, the waves split the keys (the chip is filled by keys alone); above, the rows.  (32 float32 rows of 256 do
-// not fit a wave's registers: two groups of 16.)
+// Rows to a group, how the waves share the work, and the workgroups, by the rows that a request has on average.  Up to 64
+// (float32: 32) the waves split the keys of 16: row groups of a request read the same keys from the L2 cache, and the chip is
+// filled by keys alone.  Above, the waves split the rows.  Requests of up to 8,192 tokens, 36 rows a head: 16 of them 20.3
+// us, split by rows 37.4 (bf16, 2 heads of 256), 22.7 and 44.0 (float16, 4 of 128); 96 of them 67.5 and 92.7, 82.6 and 187.
+// 60 rows, 96 requests: bf16 106 and 99, 112 and 102 (128), 76 and 87 (64), float16 130 and 197; 16 requests: 23.7 and 38.9.
+// float32, 36 rows: 36.7 and 33.1.
 struct Shape {
-  int kind, rows, workers;                       // kind 0: 16 rows, keys split; 1: 32 rows, keys split; 2: rows split
+  bool keys;                                     // the waves split the keys
+  int rows, workers;
 };
 template <typename T, int D>
 static Shape shape_of(int64_t T_, int64_t B, int64_t G) {
   constexpr int TERMS = terms_of<T>();
-  constexpr bool WIDE = TERMS == 3 && D == 256;
-  const int64_t rows = (T_ + B - 1) / B * G;
-  if (rows <= (WIDE ? 32 : 16)) return {0, 16, 256 * waves_for(D, TERMS)};
-  if (rows <= 32) return {1, 32, 256};
-  if constexpr (TERMS == 1 && D >= 128) return {2, Prompt<D>::R, 256 * prompt_waves(D)};
-  return {2, 16 * AT_WAVES * blocks_of(D, TERMS), 256 * row_waves(D, TERMS)};
+  if ((T_ + B - 1) / B * G <= (TERMS < 3 ? 64 : 32)) return {true, 16, 256 * key_waves(D, TERMS)};
+  if constexpr (TERMS == 1 && D >= 128) return {false, Prompt<D>::R, 256 * prompt_waves(D)};
+  return {false, 16 * AT_WAVES * row_blocks(D, TERMS), 256 * row_waves(D, TERMS)};
 }
 static Shape shape_for(int64_t T, int64_t B, int64_t G, int64_t D, int32_t dtype) {
   const int t = dtype == MACAI_GDR_F32 ? 0 : dtype == MACAI_GDR_BF16 ? 1 : 2;
@@ -1231,23 +1294,17 @@ static Shape shape_for(int64_t T, int64_t B, int64_t G, int64_t D, int32_t dtype
 
 template <typename T, int D>
 static void launch(const Shape& s, const AttnArgs& a, hipStream_t st) {
-  const unsigned parts = s.rows / 16 * (s.kind < 2 ? D / 32 : D < 128 ? 1 : D / 128);   // of a joined row group, a block each
+  const unsigned parts = s.rows / 16 * (s.keys ? D / 32 : D < 128 ? 1 : D / 128);   // of a joined row group, a block each
   const dim3 grid((unsigned)a.workers), threads(64 * AT_WAVES), join((unsigned)a.workers, parts);
-  if (s.kind == 0) {
-    hipLaunchKernelGGL((attend_kernel<T, D, 1, true>), grid, threads, 0, st, a);
+  if (s.keys) {
+    hipLaunchKernelGGL((attend_kernel<T, D, true>), grid, threads, 0, st, a);
     hipLaunchKernelGGL((join_many_kernel<T, D, 16>), join, dim3(256), 0, st, a);
-  } else if (s.kind == 1) {
-    if constexpr (terms_of<T>() < 3 || D < 256) {
-      hipLaunchKernelGGL((attend_kernel<T, D, 2, true>), grid, threads, 0, st, a);
-      hipLaunchKernelGGL((join_many_kernel<T, D, 32>), join, dim3(256), 0, st, a);
-    }
   } else if constexpr (std::is_same<T, bf16>::value && D >= 128) {
     hipLaunchKernelGGL((prompt_kernel<D>), grid, threads, 0, st, a);
     hipLaunchKernelGGL((join_kernel<T, D, Prompt<D>::R>), join, dim3(64), 0, st, a);
   } else {
-    constexpr int NQ = blocks_of(D, terms_of<T>());
-    hipLaunchKernelGGL((attend_kernel<T, D, NQ, false>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 16 * AT_WAVES * NQ>), join, dim3(64), 0, st, a);
+    hipLaunchKernelGGL((attend_kernel<T, D, false>), grid, threads, 0, st, a);
+    hipLaunchKernelGGL((join_kernel<T, D, 16 * AT_WAVES * row_blocks(D, terms_of<T>())>), join, dim3(64), 0, st, a);
   }
 }
 

@@ -127,6 +127,18 @@ def test_page_bytes_are_the_documented_ones(D):
                 assert value == float(x[t, 0, c]), (which, t, c)
 
 
+@pytest.mark.parametrize("T", [4095, 4096, 5001, 9000])
+def test_reading_many_rows(T):
+    """Rows in any number come out as they do in calls of a few; slots outside of the cache among them."""
+    gen = torch.Generator().manual_seed(22)
+    cache = torch.randint(0, 128, (200, 2, 1, 32 * 17 * 64 // 32), generator=gen, dtype=torch.uint8).cuda()
+    slots = torch.randint(-2, 200 * 32 + 2, (T,), generator=gen).cuda()
+    k, v = kv4_read(cache, slots, 64)
+    for a in range(0, T, 1000):
+        few = kv4_read(cache, slots[a:a + 1000], 64)
+        assert torch.equal(k[a:a + 1000], few[0]) and torch.equal(v[a:a + 1000], few[1]), a
+
+
 def test_append_extremes():
     """Ties, the smallest and largest scales, zeros, and groups that hold an infinity or a NaN (they alone read as NaN)."""
     x = torch.zeros(8, 1, 64)
@@ -230,6 +242,22 @@ def test_long_contexts_split_over_the_chip(B, lens, qlen, G, D, Hk):
     _against_oracle(o, q, ks, vs, lens, [qlen] * B, BF16)
     for _ in range(3):
         assert torch.equal(kv4_attention(*args), o)                       # the same bits every time
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("B,Hk,G,D,ctx,most", [(3, 2, 8, 128, 700, 7), (60, 8, 6, 256, 40, 5), (70, 1, 8, 64, 200, 6),
+                                               (64, 2, 8, 128, 90, 4), (6, 1, 16, 256, 1500, 4), (130, 2, 4, 64, 30, 1)])
+def test_requests_of_several_row_groups(B, Hk, G, D, ctx, most, dtype):
+    """Few requests, whose row groups are cut apart from each other, and many, whose row groups share workgroups: with and
+    without queries, with fewer tokens than queries, and with none."""
+    rng = random.Random(B)
+    lens = [0, 1, ctx] + [rng.randint(0, ctx) for _ in range(B - 3)]
+    qlens = [most, most, most] + [rng.randint(0, most) for _ in range(B - 3)]
+    cache, blocks, _, ks, vs, gen = _setup(lens, Hk, D, 16, dtype, 21)
+    q = torch.randn(sum(qlens), Hk * G, D, generator=gen).to(dtype)
+    starts = torch.tensor([0] + qlens).cumsum(0).to(torch.int32).cuda()
+    o = kv4_attention(q.cuda(), cache, blocks, torch.tensor(lens, **I32), starts)
+    _against_oracle(o, q, ks, vs, lens, qlens, dtype)
 
 
 def test_scores_that_grow_along_the_keys():
