@@ -243,6 +243,13 @@ struct AppendArgs {
   int Hq, Hk, D, page, page_shift;
 };
 
+// Which of `count` rows (or runs of rows) block b of as many takes.  Blocks go to the 8 dies in turn, and neighbouring rows
+// mostly share lines of the cache: 16 neighbours are given to blocks of one die, whose L2 puts their lines together.
+__device__ __forceinline__ unsigned on_one_die(unsigned b, unsigned count) {
+  const unsigned i = b >> 3;
+  return b >= count / 128 * 128 ? b : (i / 16 * 8 + (b & 7)) * 16 + i % 16;
+}
+
 // The largest of 4 neighbouring lanes (two exchanges inside the quad).
 __device__ __forceinline__ unsigned quad_max(unsigned x) {
   x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, true));
@@ -251,7 +258,8 @@ __device__ __forceinline__ unsigned quad_max(unsigned x) {
 
 // A thread takes 8 channels of one head of q, k or v of a row, its loads issued before the first use; 4 neighbours hold a
 // group of 32.  Rotated channels of the half layout load their partners too (from the first-level cache: another thread's
-// own).  16,383 tokens, 32 + 2 x 8 heads of 128, bf16: 79 us, 4.7 TB/s (two rows a thread 79, four 88).  A q of APPEND_PAST
+// own).  16,383 tokens, 32 + 2 x 8 heads of 128, bf16: 79.5 us, 382 MB at 4.8 TB/s, near a copy's rate (block after block,
+// neighbours on 8 dies, 37 MB more of parts of lines and 82.5 us; two rows a thread the same, four 88).  A q of APPEND_PAST
 // values or more, past what the L2 caches hold, is written past them (79 against 87 us).
 constexpr int64_t APPEND_PAST = INT64_C(1) << 24;
 template <typename T, bool PAST>
@@ -259,7 +267,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
   const int per = a.D / 8, heads = a.Hq + 2 * a.Hk;
   const int vec = blockIdx.y * 256 + threadIdx.x;
   if (vec >= heads * per) return;
-  const int64_t row = blockIdx.x;
+  const int64_t row = on_one_die(blockIdx.x, gridDim.x);
   const int ch = vec % per * 8;
   int h = vec / per;
   const int which = h < a.Hq ? 0 : h < a.Hq + a.Hk ? 1 : 2;
@@ -333,8 +341,8 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
 
 // Slots' keys and values as T [rows, heads, D] each: 8 channels a thread, whole rows a block, so that a thread's place is
 // one 32-bit division; a slot outside of the cache reads as zeros.  Neighbouring rows mostly share lines of the cache: with
-// many rows a block takes 4 at least, and 16 neighbouring blocks are blocks of one die, whose L2 holds a line for all of
-// them (16,383 rows of 8 heads of 128: 20.4 us, 4.1 TB/s; 28.5 a row a block and block after block, 22.5 with the dies alone).
+// many rows a block takes 4 at least (16,383 rows of 8 heads of 128: 20.4 us, 4.1 TB/s; a row a block 22.5, and block after
+// block on 8 dies 28.5).
 // With few rows what counts is how many threads there are (64 rows: 2.7 us a row a block, 3.5 four).
 constexpr int64_t READ_MANY = 4096;
 template <typename T>
@@ -374,8 +382,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) read_kernel(const uint8_t* cache, const int64_t* slots, T* k, T* v, int64_t rows,
                                                    int64_t pages, int Hk, int D, int page, int page_shift, int block_rows) {
   const int shift = __builtin_ctz(D / 8), pieces = 2 * Hk << shift;
-  const int64_t i16 = blockIdx.x >> 3;           // blocks go to the 8 dies in turn
-  const int64_t block = blockIdx.x >= gridDim.x / 128 * 128 ? blockIdx.x : (i16 / 16 * 8 + (blockIdx.x & 7)) * 16 + i16 % 16;
+  const int64_t block = on_one_die(blockIdx.x, gridDim.x);
   for (int i = threadIdx.x; i < block_rows * pieces; i += 256) {
     const int r = (unsigned)i / (unsigned)pieces, c = i - r * pieces;
     const int64_t row = block * block_rows + r;
