@@ -654,6 +654,10 @@ constexpr int row_waves(int D, int terms) { return D == 64 || (terms == 3 && D =
 
 // KEYS: the workgroup's waves take different keys of the same 16 rows and join their results at the end (few rows);
 // else different rows of the same keys (16 NQ each).
+// Bound by the cache's bytes where contexts are long (bf16; 64 requests of up to 32,768 tokens, 2 heads of 256: 380 MB in 75
+// us, 5.1 TB/s; one of 262,144, 8 heads of 128: 285 MB in 54.5 us, 5.2 TB/s), by its chain of loads where they are short
+// (lengths, page number, tile: 517 tokens 7.7 us, of which finding the stretch 1.8, the tile with its page 3, the join 1.2).
+// The join was two exchanges between pairs of waves before: 1.9 us.
 template <typename T, int D, bool KEYS>
 __global__ void __launch_bounds__(64 * AT_WAVES, KEYS ? key_waves(D, terms_of<T>()) : row_waves(D, terms_of<T>()))
     attend_kernel(AttnArgs a) {
@@ -751,7 +755,11 @@ __global__ void __launch_bounds__(64 * AT_WAVES, KEYS ? key_waves(D, terms_of<T>
 //            group of 32 channels and term: exact for values down to 2^-13 of their group's largest, 2^-21 of the largest
 //            below.  Two such products of 128 channels take half the time of the four bf16 ones.
 //   values   decoded once for the workgroup, a quarter each, into LDS in the order that the second product's operand has
-//            (contiguous 16-byte reads, no bank conflict); two buffers, one barrier a tile.
+//            (contiguous 16-byte reads, no bank conflict); two buffers, one barrier a tile.  (The 8-byte writes meet two
+//            at a bank; with an operand's halves apart they did not, and it took 211 us for 208.)
+// 4 requests, up to 1,024 queries of 16 heads of 256 over up to 8,192 tokens: 182 GFLOP in 205 us.  The matrix cores are
+// busy in 178 thousand of its 410 thousand clocks; the rest is softmax and decoding that the other workgroup's products do
+// not cover, 13 us to begin and end each row group, and the parts of split ones (111 MB).
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
 template <int D>
@@ -980,8 +988,8 @@ struct Prompt {
         }
   }
 
-  // O^T += V^T P^T from a buffer of operands, four fragments in flight (two took 128 us where four take 125, at heads of 128; heads of
-  // 256 have registers for two).
+  // O^T += V^T P^T from a buffer of operands, four fragments in flight (two took 128 us where four take 126, at heads of
+  // 128; heads of 256 have registers for two).
   __device__ __forceinline__ void values(const unsigned (*buf)[64][4], const bf16x8 (&p)[NQ][KB], int lane) {
     constexpr int N = KB * ND, AHEAD = D == 256 ? 2 : 4;
     u32x4_t v[AHEAD];
@@ -1162,7 +1170,7 @@ struct Join {
   }
 };
 
-// Few parts (row groups of many rows, a wave a block).
+// Few parts (row groups of many rows, a wave a block): a stream, 58 MB in 20 us where 4 prompts' row groups were split.
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(64) join_kernel(AttnArgs a) {
   constexpr int TILES = D < 128 ? D / 16 : 8;
@@ -1198,7 +1206,8 @@ __global__ void __launch_bounds__(64) join_kernel(AttnArgs a) {
 }
 
 // Many parts: one long context leaves a few rows with a hundred of them.  What counts is how many lines are in flight, on
-// how many CUs: a block takes two tiles, a wave a part in 4, BATCH of them at once, and the waves join through LDS.
+// how many CUs: a block takes two tiles, a wave a part in 4, BATCH of them at once, and the waves join through LDS (one
+// request of 262,144 tokens 6.9 us, 64 of up to 32,768 7.7, of 517 3.4: a launch and two loads that wait for each other).
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(256) join_many_kernel(AttnArgs a) {
   using JT = Join<T, D, R, 2>;

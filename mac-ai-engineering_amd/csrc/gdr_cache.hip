@@ -149,6 +149,7 @@ struct PlanArgs {
 // One launch: every workgroup sums over all requests (PLAN_REQ at a time) and finds its own 256 tokens among them, so that
 // nothing waits for another workgroup.  A page is taken by the token that begins it, which also enters it in the table;
 // tokens on a page that was there before read the table, whose old entries no workgroup writes.
+// Bound by its latency: 64 requests of one token 4.6 us, 256 of up to 512 tokens (754 KB) 6.2.
 constexpr int PLAN_REQ = 1024;
 __global__ void __launch_bounds__(256) plan_kernel(PlanArgs a) {
   __shared__ int64_t first[PLAN_REQ + 1];      // where a request's tokens begin
