@@ -505,7 +505,8 @@ struct Rows {
   // Masks the keys that rows do not see and clears the values past kend and those that read as NaN (0 times NaN is not 0:
   // a NaN goes to the rows that see it by itself).  nan: bit m of [b][c] is set where the row sees a NaN in the group that
   // lanes m load of chunk c.
-  __device__ __forceinline__ void hide(KvTile<D>& t, f4 (&s)[NQ][2], unsigned (&nan)[NQ][KvTile<D>::NC], int t0, int kend, int h) {
+  __device__ __forceinline__ void hide(KvTile<D>& t, f4 (&s)[NQ][2], unsigned (&nan)[NQ][KvTile<D>::NC], int t0, int kend,
+                                       int h) {
 #pragma unroll
     for (int b = 0; b < NQ; ++b)
 #pragma unroll
@@ -886,7 +887,8 @@ struct Prompt {
                                                       bool masked, int kend, int lane) {
     const int h = lane >> 4, u = wave / NC, c = wave % NC;
     const u32x4_t codes = *reinterpret_cast<const u32x4_t*>(&raw.v[wave][lane][0]);
-    unsigned vs = *reinterpret_cast<const unsigned*>(&raw.scales[u * NC][D / 2 + h * (D / 8) + (4 * c + ((lane & 15) >> 2)) * 4]);
+    const int group = 4 * c + ((lane & 15) >> 2);
+    unsigned vs = *reinterpret_cast<const unsigned*>(&raw.scales[u * NC][D / 2 + h * (D / 8) + group * 4]);
     unsigned vc[4] = {codes[0], codes[1], codes[2], codes[3]};
     if (masked) {
 #pragma unroll
@@ -949,7 +951,8 @@ struct Prompt {
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
         const i32x8_t k = {(int)x[u][0], (int)x[u][1], (int)x[u][2], (int)x[u][3], 0, 0, 0, 0};
-        s[b][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q[b][C % NC][1], s[b][u], 4, 0, 0, ks[u], 2 * C + 1, (int)qs[b]);
+        s[b][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q[b][C % NC][1], s[b][u], 4, 0, 0, ks[u], 2 * C + 1,
+                                                                   (int)qs[b]);
       }
   }
 
@@ -1286,38 +1289,53 @@ __global__ void __launch_bounds__(256) join_many_kernel(AttnArgs a) {
 // us, split by rows 37.4 (bf16, 2 heads of 256), 22.7 and 44.0 (float16, 4 of 128); 96 of them 67.5 and 92.7, 82.6 and 187.
 // 60 rows, 96 requests: bf16 106 and 99, 112 and 102 (128), 76 and 87 (64), float16 130 and 197; 16 requests: 23.7 and 38.9.
 // float32, 36 rows: 36.7 and 33.1.
+//
+// A row group that is split over some workgroups leaves a part in each, which a wave takes one after the other in 4 us
+// each; the waves that share them take as long for a whole launch as the parts are many bytes in small pieces.  With 16
+// workgroups to a row group (16 requests of up to 8,192 tokens, 100 rows, 2 heads of 256) 62 us and 26, with 4 (one request
+// of 8,192, 8,192 rows) 20 and 51; they meet at about 8 (10, heads of 64: 14 and 7.6).
 struct Shape {
   bool keys;                                     // the waves split the keys
   int rows, workers;
+  bool many;                                     // many parts to a row group
 };
 template <typename T, int D>
-static Shape shape_of(int64_t T_, int64_t B, int64_t G) {
+static Shape shape_of(int64_t T_, int64_t B, int64_t G, int64_t Hk) {
   constexpr int TERMS = terms_of<T>();
-  if ((T_ + B - 1) / B * G <= (TERMS < 3 ? 64 : 32)) return {true, 16, 256 * key_waves(D, TERMS)};
-  if constexpr (TERMS == 1 && D >= 128) return {false, Prompt<D>::R, 256 * prompt_waves(D)};
-  return {false, 16 * AT_WAVES * row_blocks(D, TERMS), 256 * row_waves(D, TERMS)};
+  const int64_t rows = (T_ + B - 1) / B * G;
+  if (rows <= (TERMS < 3 ? 64 : 32)) return {true, 16, 256 * key_waves(D, TERMS), true};
+  Shape s{false, 16 * AT_WAVES * row_blocks(D, TERMS), 256 * row_waves(D, TERMS), false};
+  if constexpr (TERMS == 1 && D >= 128) s = {false, Prompt<D>::R, 256 * prompt_waves(D), false};
+  s.many = (rows + s.rows - 1) / s.rows * B * Hk * 8 <= s.workers;
+  return s;
 }
-static Shape shape_for(int64_t T, int64_t B, int64_t G, int64_t D, int32_t dtype) {
-  const int t = dtype == MACAI_GDR_F32 ? 0 : dtype == MACAI_GDR_BF16 ? 1 : 2;
-  const Shape all[3][3] = {{shape_of<float, 64>(T, B, G), shape_of<float, 128>(T, B, G), shape_of<float, 256>(T, B, G)},
-                           {shape_of<bf16, 64>(T, B, G), shape_of<bf16, 128>(T, B, G), shape_of<bf16, 256>(T, B, G)},
-                           {shape_of<f16, 64>(T, B, G), shape_of<f16, 128>(T, B, G), shape_of<f16, 256>(T, B, G)}};
-  return all[t][D == 64 ? 0 : D == 128 ? 1 : 2];
+static Shape shape_for(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int32_t dtype) {
+  const auto of = [&](auto type) {
+    using PT = decltype(type);
+    const int64_t G = Hq / Hk;
+    return D == 64 ? shape_of<PT, 64>(T, B, G, Hk) : D == 128 ? shape_of<PT, 128>(T, B, G, Hk) : shape_of<PT, 256>(T, B, G, Hk);
+  };
+  return dtype == MACAI_GDR_F32 ? of(0.f) : dtype == MACAI_GDR_BF16 ? of((bf16)0.f) : of((f16)0.f);
 }
 
+template <typename T, int D, int R>
+static void launch_join(const Shape& s, const AttnArgs& a, hipStream_t st) {
+  const dim3 join((unsigned)a.workers, (unsigned)(R / 16 * (s.many ? D / 32 : D < 128 ? 1 : D / 128)));   // a row group's blocks
+  if (R == 16 || s.many) hipLaunchKernelGGL((join_many_kernel<T, D, R>), join, dim3(256), 0, st, a);
+  else if constexpr (R > 16) hipLaunchKernelGGL((join_kernel<T, D, R>), join, dim3(64), 0, st, a);
+}
 template <typename T, int D>
 static void launch(const Shape& s, const AttnArgs& a, hipStream_t st) {
-  const unsigned parts = s.rows / 16 * (s.keys ? D / 32 : D < 128 ? 1 : D / 128);   // of a joined row group, a block each
-  const dim3 grid((unsigned)a.workers), threads(64 * AT_WAVES), join((unsigned)a.workers, parts);
+  const dim3 grid((unsigned)a.workers), threads(64 * AT_WAVES);
   if (s.keys) {
     hipLaunchKernelGGL((attend_kernel<T, D, true>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_many_kernel<T, D, 16>), join, dim3(256), 0, st, a);
+    launch_join<T, D, 16>(s, a, st);
   } else if constexpr (std::is_same<T, bf16>::value && D >= 128) {
     hipLaunchKernelGGL((prompt_kernel<D>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, Prompt<D>::R>), join, dim3(64), 0, st, a);
+    launch_join<T, D, Prompt<D>::R>(s, a, st);
   } else {
     hipLaunchKernelGGL((attend_kernel<T, D, false>), grid, threads, 0, st, a);
-    hipLaunchKernelGGL((join_kernel<T, D, 16 * AT_WAVES * row_blocks(D, terms_of<T>())>), join, dim3(64), 0, st, a);
+    launch_join<T, D, 16 * AT_WAVES * row_blocks(D, terms_of<T>())>(s, a, st);
   }
 }
 
@@ -1334,7 +1352,7 @@ extern "C" {
 
 int64_t macai_gdr_kv4_attention_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int32_t dtype) {
   if (T < 1 || B < 1 || Hk < 1 || Hq < Hk || D < 1) return 0;
-  const gdr::Shape s = gdr::shape_for(T, B, Hq / Hk, D, dtype);
+  const gdr::Shape s = gdr::shape_for(T, B, Hq, Hk, D, dtype);
   return s.workers * (int64_t)(2 * sizeof(int4) + 2 * s.rows * (D + 4) * sizeof(float));
 }
 
@@ -1362,7 +1380,7 @@ int macai_gdr_kv4_attention(const void* q, const uint8_t* cache, const int32_t* 
     if (!aligned16(p)) return fail(MACAI_GDR_EINVAL, "%s: pointers must be 16-byte aligned", what);
   const int64_t v = dtype == MACAI_GDR_F32 ? 4 : 8;
   if (q_row % v || q_head % v) return fail(MACAI_GDR_EINVAL, "%s: strides must keep 16-byte alignment", what);
-  const gdr::Shape s = gdr::shape_for(T, B, Hq / Hk, D, dtype);
+  const gdr::Shape s = gdr::shape_for(T, B, Hq, Hk, D, dtype);
   gdr::AttnArgs a{q, o, cache, blocks, lens, starts, nullptr, nullptr, q_row, q_head, T, B, W, pages, (int)Hq, (int)Hk,
                   (int)page, __builtin_ctzll((unsigned long long)page), s.workers, scale * 1.44269504088896341f};
   a.records = (int4*)workspace;

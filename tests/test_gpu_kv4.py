@@ -245,6 +245,20 @@ def test_long_contexts_split_over_the_chip(B, lens, qlen, G, D, Hk):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("B,Hk,G,D,ctx,most", [(12, 3, 8, 128, 300, 60), (10, 2, 8, 256, 200, 70), (9, 4, 10, 64, 260, 50)])
+def test_many_row_groups_of_prompts(B, Hk, G, D, ctx, most, dtype):
+    """More row groups than an eighth of the workgroups: few parts to a row group, most of them whole."""
+    rng = random.Random(B)
+    qlens = [most] + [rng.randint(most // 2, most) for _ in range(B - 1)]
+    lens = [n + rng.randint(0, ctx) for n in qlens]
+    cache, blocks, _, ks, vs, gen = _setup(lens, Hk, D, 32, dtype, 23)
+    q = torch.randn(sum(qlens), Hk * G, D, generator=gen).to(dtype)
+    starts = torch.tensor([0] + qlens).cumsum(0).to(torch.int32).cuda()
+    o = kv4_attention(q.cuda(), cache, blocks, torch.tensor(lens, **I32), starts)
+    _against_oracle(o, q, ks, vs, lens, qlens, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("B,Hk,G,D,ctx,most", [(3, 2, 8, 128, 700, 7), (60, 8, 6, 256, 40, 5), (70, 1, 8, 64, 200, 6),
                                                (64, 2, 8, 128, 90, 4), (6, 1, 16, 256, 1500, 4), (130, 2, 4, 64, 30, 1)])
 def test_requests_of_several_row_groups(B, Hk, G, D, ctx, most, dtype):
